@@ -190,7 +190,8 @@ def _handle(state):
         c4s = _package()
         state["ctx"] = c4s.SamplingContext(max_vocab=64, device=_device().index, max_rows=1)
         if "k" in state:
-            state["cache"] = c4s.KVCache(state["k"], state["v"], state["k_sb"], state["v_sb"])
+            state["cache"] = c4s.KVCache(state["k"], state["v"], state["k_sb"], state["v_sb"],
+                                         bits=state["case"]["bits"])
         if state["op"] == "attention":
             state["work"] = state["ctx"].attention_workspace(state["q"].shape[0], state["q"].shape[1],
                                                              state["q"].shape[2])
