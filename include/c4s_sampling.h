@@ -89,6 +89,8 @@ typedef struct c4s_row_params {
 #define C4S_DEVERR_TIMEOUT 2u    /* a bounded wait on a bulk copy gave up      */
 #define C4S_DEVERR_HIST_FULL 8u  /* c4s_decode_step: a row's history window was full
                                     (or its id outside the embedding); the row stopped */
+#define C4S_DEVERR_KV_PAGE 16u /* a cache position past its page table's width, or a page
+                                    number outside the cache: the position was left out  */
 #define C4S_DEVERR_SHARD 4u      /* vocab-sharded merge: a row it cannot decide
                                     exactly (top_k outside [1, 64], or more than
                                     64 of a shard's values tied at the top_k
@@ -217,6 +219,87 @@ int c4s_quantize_affine(c4s_ctx* ctx, const float* d_w, int32_t N, int32_t K, in
 int c4s_qgemv(c4s_ctx* ctx, const float* d_x, int32_t B, int32_t K, const uint32_t* d_q, const float* d_scales,
               const float* d_biases, int32_t N, int32_t group, int32_t bits, const float* d_bias_out, float* d_y,
               void* stream);
+
+/* ------------------------------------------------------------------------
+ * The key-value cache of the GPT-2 blocks and the attention that reads it.
+ * The reference grows a dense cache per layer by concatenation and attends
+ * over it with MLX's fused attention (gpt2.cpp, forward with a cache; batches
+ * are left-padded and masked, text2semantic.cpp:196-373). Here the cache is a
+ * pool of pages that sequences own through a page table, so that a batch
+ * needs no padding and nothing is copied as it grows.
+ *
+ * A cache holds, for keys and for values alike, one row of head_dim elements
+ * per (page, kv head, slot): page_size slots to a page, addressed by three
+ * strides in bytes, so pages may be [head][slot] or [slot][head]. Rows are
+ *   bits 16   bf16 or fp16 elements (dtype), or
+ *   bits 8/4  codes of the affine scheme of c4s_quantize_affine in groups of
+ *             `group` elements (32 or 64), element 2i in the low half of byte
+ *             i for 4 bits, with one fp32 pair (scale, bias) per group at
+ *             k_sb / v_sb (same addressing, strides of its own): value =
+ *             scale code + bias. The code is the integer nearest to
+ *             (x - min) (2^bits - 1) / (max - min), ties to even, decided
+ *             exactly; a group with a NaN or infinity reads back as NaN.
+ * k and v share the strides. head_dim 64, 96 or 128, divided by the group;
+ * row addresses and strides multiples of 16 bytes, of pairs 8 bytes.
+ *
+ * d_page_table: int32 [B, max_pages], rows table_ld apart. Position p of
+ * sequence b is slot p % page_size of page d_page_table[b][p / page_size];
+ * entries behind a sequence's last page are not read. A position past the
+ * table, or on a page outside [0, num_pages), is left out of every operation
+ * and sets C4S_DEVERR_KV_PAGE. Pages may be shared by sequences that only
+ * read them; two sequences that write one page must not share a slot.      */
+typedef enum c4s_dtype { C4S_BF16 = 0, C4S_FP16 = 1, C4S_FP32 = 2 } c4s_dtype;
+typedef struct c4s_kv_cache {
+  void* k;
+  void* v;
+  float* k_sb;                /* (scale, bias) pairs; NULL for bits 16 */
+  float* v_sb;
+  int64_t page_stride, head_stride, token_stride;            /* bytes */
+  int64_t sb_page_stride, sb_head_stride, sb_token_stride;   /* bytes */
+  int32_t num_pages, page_size, kv_heads, head_dim;
+  int32_t bits, dtype, group;
+} c4s_kv_cache;
+
+/* Write new tokens' keys and values: d_k, d_v [T, kv_heads, head_dim] of
+ * `dtype` (bf16 or fp16; the cache's for bits 16), rows of head_dim contiguous
+ * elements, token_stride and head_stride in elements (slices of a fused
+ * projection need no copy). With d_tok_off (int64 [B+1]) the tokens
+ * [off[b], off[b+1]) are sequence b's and go to positions d_pos[b],
+ * d_pos[b] + 1, ...; with NULL token b is sequence b's (T = B), the decode
+ * step. A sequence with d_pos[b] < 0 is skipped; tokens behind off[B] are not
+ * read. Replaces the cache's concatenation in gpt2.cpp's forward.          */
+int c4s_kv_write(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* d_page_table, int64_t table_ld,
+                 int32_t max_pages, int32_t B, const void* d_k, const void* d_v, int32_t dtype,
+                 int64_t token_stride, int64_t head_stride, int64_t T, const int64_t* d_tok_off,
+                 const int32_t* d_pos, void* stream);
+
+/* Read positions back: the inverse of c4s_kv_write, with the same arguments;
+ * d_k, d_v are written, of any c4s_dtype. Rows of skipped sequences and
+ * behind off[B] are left as they were; positions left out read as zeros.   */
+int c4s_kv_read(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* d_page_table, int64_t table_ld,
+                int32_t max_pages, int32_t B, void* d_k, void* d_v, int32_t dtype, int64_t token_stride,
+                int64_t head_stride, int64_t T, const int64_t* d_tok_off, const int32_t* d_pos, void* stream);
+
+/* Attention of one new token per sequence over the cache:
+ *   out[b, h] = sum_p softmax_p(scale q[b, h] . k[p, h / G]) v[p, h / G],
+ *   p in [d_start[b], d_len[b]), G = q_heads / kv_heads
+ * (d_start NULL: from 0; a later start is a left-padded prompt's mask or a
+ * sliding window). A sequence with nothing visible (length 0 or negative, or
+ * start >= length) gets zeros. q, out [B, q_heads, head_dim] of `dtype` (bf16
+ * or fp16; the cache's for bits 16), rows contiguous, strides in elements.
+ * Lengths are read on the device, so the call can be captured while they
+ * grow. Scores, softmax and sums are fp32; P is not rounded to 16 bits.
+ * d_work: caller-owned device workspace, 16-byte aligned, of at least
+ * c4s_attention_workspace(ctx, B, q_heads, head_dim) bytes, zeroed once
+ * before its first use (each call leaves it ready for the next); calls that
+ * may overlap in time need workspaces of their own.
+ * Replaces the fused attention call of gpt2.cpp's decode step.             */
+int64_t c4s_attention_workspace(c4s_ctx* ctx, int32_t B, int32_t q_heads, int32_t head_dim);
+int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* d_page_table, int64_t table_ld,
+                        int32_t max_pages, int32_t B, const void* d_q, int32_t dtype, int32_t q_heads,
+                        int64_t q_batch_stride, int64_t q_head_stride, const int32_t* d_len, const int32_t* d_start,
+                        float scale, void* d_out, int64_t out_batch_stride, int64_t out_head_stride, void* d_work,
+                        int64_t work_bytes, void* stream);
 
 /* Apply the processors selected by `stages` (C4S_STAGE_* bits) in place to B
  * rows of d_logits, in the reference order, ignoring params.greedy.

@@ -1,0 +1,267 @@
+// c4s_block.cu -- C ABI of the decoder block's operators: the paged key-value
+// cache (c4s_kv.cuh) and the attention over it (c4s_attn.cuh).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <type_traits>
+
+#include "c4s_context.cuh"
+#include "c4s_device.cuh"
+#include "c4s_kvidx.cuh"
+#include "c4s_kv.cuh"
+#include "c4s_attn.cuh"
+
+namespace {
+
+// Launch with programmatic stream serialisation (every kernel here waits in
+// grid_dep_wait before it touches what earlier launches wrote).
+template <typename... P, typename... A>
+cudaError_t launch(void (*kern)(P...), dim3 grid, int block, size_t smem, void* stream, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...);
+}
+
+// The checks of a cache and its page table that every entry point makes.
+const char* bad_cache(const c4s_kv_cache* c, const int32_t* table, int64_t table_ld, int32_t max_pages, int32_t B) {
+  if (!c || !c->k || !c->v || !table) return "null pointer";
+  if (c->num_pages < 1 || c->page_size < 1 || c->kv_heads < 1 || c->kv_heads > 65535 || max_pages < 1)
+    return "num_pages, page_size, kv_heads and max_pages must be positive";
+  if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128) return "head_dim must be 64, 96 or 128";
+  if (c->bits != 16 && c->bits != 8 && c->bits != 4) return "bits must be 16, 8 or 4";
+  if (((uintptr_t)c->k & 15) || ((uintptr_t)c->v & 15) || (c->page_stride & 15) || (c->head_stride & 15) ||
+      (c->token_stride & 15))
+    return "cache rows must start on 16 bytes";
+  if (c->page_stride < 0 || c->head_stride < 0 || c->token_stride < 0) return "negative cache stride";
+  if (c->bits == 16) {
+    if (c->dtype != C4S_BF16 && c->dtype != C4S_FP16) return "16-bit cache rows are bf16 or fp16";
+  } else {
+    if ((c->group != 32 && c->group != 64) || c->head_dim % c->group) return "group must be 32 or 64 and divide head_dim";
+    if (!c->k_sb || !c->v_sb) return "scales and biases missing";
+    if (((uintptr_t)c->k_sb & 7) || ((uintptr_t)c->v_sb & 7) || (c->sb_page_stride & 7) || (c->sb_head_stride & 7) ||
+        (c->sb_token_stride & 7))
+      return "scale and bias pairs must start on 8 bytes";
+    if (c->sb_page_stride < 0 || c->sb_head_stride < 0 || c->sb_token_stride < 0) return "negative cache stride";
+  }
+  if (B > 1 && table_ld < max_pages) return "table_ld < max_pages";
+  return nullptr;
+}
+
+c4s::KvCache view(const c4s_kv_cache* c) {
+  c4s::KvCache v;
+  v.k = static_cast<unsigned char*>(c->k);
+  v.v = static_cast<unsigned char*>(c->v);
+  v.k_sb = reinterpret_cast<unsigned char*>(c->k_sb);
+  v.v_sb = reinterpret_cast<unsigned char*>(c->v_sb);
+  v.page_stride = c->page_stride;
+  v.head_stride = c->head_stride;
+  v.token_stride = c->token_stride;
+  v.sb_page_stride = c->sb_page_stride;
+  v.sb_head_stride = c->sb_head_stride;
+  v.sb_token_stride = c->sb_token_stride;
+  v.num_pages = c->num_pages;
+  v.page_size = c->page_size;
+  v.heads = c->kv_heads;
+  v.dim = c->head_dim;
+  v.group = c->bits == 16 ? 64 : c->group;
+  return v;
+}
+
+// Common part of c4s_kv_write and c4s_kv_read: checks and arguments.
+int kv_args(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* table, int64_t table_ld, int32_t max_pages,
+            int32_t B, const void* k, const void* v, int32_t dtype, int64_t tstride, int64_t hstride, int64_t T,
+            const int64_t* off, const int32_t* pos, c4s::KvArgs& a, unsigned& grid) {
+  if (B < 0 || T < 0) return fail(ctx, C4S_ERR_INVALID, "B < 0 or T < 0");
+  grid = 0;
+  if (!off && T != B) return fail(ctx, C4S_ERR_INVALID, "without offsets T must be B (one token per sequence)");
+  if (B == 0 || T == 0) return C4S_OK;
+  if (const char* why = bad_cache(cache, table, table_ld, max_pages, B)) return fail(ctx, C4S_ERR_INVALID, why);
+  if (!k || !v || !pos) return fail(ctx, C4S_ERR_INVALID, "null pointer");
+  if (tstride < 0 || hstride < 0) return fail(ctx, C4S_ERR_INVALID, "negative stride");
+  const uintptr_t es = dtype == C4S_FP32 ? 4 : 2;
+  if (((uintptr_t)k | (uintptr_t)v) & (es - 1)) return fail(ctx, C4S_ERR_INVALID, "misaligned rows");
+  const long long units = (long long)cache->kv_heads * (cache->head_dim / 8);
+  if (T > 0x7fffffffLL * c4s::KV_NT / units - 1) return fail(ctx, C4S_ERR_CAPACITY, "too many tokens in one call");
+  grid = (unsigned)((T * units + c4s::KV_NT - 1) / c4s::KV_NT);
+  a.c = view(cache);
+  a.table = table;
+  a.table_ld = table_ld;
+  a.max_pages = max_pages;
+  a.B = B;
+  a.k = k;
+  a.v = v;
+  a.tstride = tstride;
+  a.hstride = hstride;
+  a.vec = ((((uintptr_t)k | (uintptr_t)v) & 15) | ((tstride * es) & 15) | ((hstride * es) & 15)) == 0;
+  a.T = T;
+  a.off = reinterpret_cast<const long long*>(off);
+  a.pos = pos;
+  a.errflags = ctx->d_err;
+  return C4S_OK;
+}
+
+using KvKernel = void (*)(c4s::KvArgs);
+
+template <typename T> KvKernel write_kernel(int bits) {
+  return bits == 16 ? c4s::kv_write_kernel<T, 16> : bits == 8 ? c4s::kv_write_kernel<T, 8> : c4s::kv_write_kernel<T, 4>;
+}
+template <typename TO> KvKernel read_kernel(int bits, int cache_dtype) {
+  if (bits == 8) return c4s::kv_read_kernel<__half, TO, 8>;
+  if (bits == 4) return c4s::kv_read_kernel<__half, TO, 4>;
+  return cache_dtype == C4S_BF16 ? c4s::kv_read_kernel<__nv_bfloat16, TO, 16> : c4s::kv_read_kernel<__half, TO, 16>;
+}
+
+using AttnKernel = void (*)(c4s::AttnArgs);
+using JoinKernel = void (*)(c4s::AttnArgs, int);
+struct AttnPick {
+  AttnKernel main = nullptr;
+  JoinKernel join = nullptr;
+  int smem = 0, tok = 0;
+};
+template <typename T, int D, int BITS, int GS, int NQ> AttnPick attn_pick() {
+  using Cfg = c4s::AttnCfg<D, BITS, GS>;
+  return {c4s::attn_kernel<T, D, BITS, GS, NQ>, c4s::attn_join_kernel<T, D, NQ>, Cfg::SMEM, Cfg::TOK};
+}
+template <typename T, int D, int NQ> AttnPick attn_pick_rows(int bits, int group) {
+  if (bits == 16) return attn_pick<T, D, 16, 32, NQ>();
+  if constexpr (D % 64 == 0) {
+    if (group == 64) return bits == 8 ? attn_pick<T, D, 8, 64, NQ>() : attn_pick<T, D, 4, 64, NQ>();
+  }
+  return bits == 8 ? attn_pick<T, D, 8, 32, NQ>() : attn_pick<T, D, 4, 32, NQ>();
+}
+template <typename T, int NQ> AttnPick attn_pick_dim(int dim, int bits, int group) {
+  return dim == 64 ? attn_pick_rows<T, 64, NQ>(bits, group)
+                   : dim == 96 ? attn_pick_rows<T, 96, NQ>(bits, group) : attn_pick_rows<T, 128, NQ>(bits, group);
+}
+
+constexpr int ATT_CTAS = 2;                        // per SM: what their shared memory is sized for
+
+int64_t attn_work_bytes(const c4s_ctx* ctx, int dim) {
+  const int64_t W = (int64_t)ctx->num_sms * ATT_CTAS * c4s::ATT_WARPS;
+  return W * 2 * 8 * (dim + 2) * 4;
+}
+
+}  // namespace
+
+extern "C" {
+
+int c4s_kv_write(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* d_page_table, int64_t table_ld,
+                 int32_t max_pages, int32_t B, const void* d_k, const void* d_v, int32_t dtype, int64_t token_stride,
+                 int64_t head_stride, int64_t T, const int64_t* d_tok_off, const int32_t* d_pos, void* stream) try {
+  if (!ctx) return C4S_ERR_INVALID;
+  c4s::KvArgs a;
+  unsigned grid;
+  if (dtype != C4S_BF16 && dtype != C4S_FP16) return fail(ctx, C4S_ERR_INVALID, "new keys and values are bf16 or fp16");
+  const int rc = kv_args(ctx, cache, d_page_table, table_ld, max_pages, B, d_k, d_v, dtype, token_stride, head_stride,
+                         T, d_tok_off, d_pos, a, grid);
+  if (rc || grid == 0) return rc;
+  if (cache->bits == 16 && dtype != cache->dtype) return fail(ctx, C4S_ERR_INVALID, "the cache's rows are of another type");
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok) return fail(ctx, C4S_ERR_CUDA, "cannot select the context's device");
+  const KvKernel kern = dtype == C4S_BF16 ? write_kernel<__nv_bfloat16>(cache->bits) : write_kernel<__half>(cache->bits);
+  const cudaError_t e = launch(kern, dim3(grid), c4s::KV_NT, 0, stream, a);
+  return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "cache write launch");
+} catch (...) {
+  return C4S_ERR_INVALID;
+}
+
+int c4s_kv_read(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* d_page_table, int64_t table_ld,
+                int32_t max_pages, int32_t B, void* d_k, void* d_v, int32_t dtype, int64_t token_stride,
+                int64_t head_stride, int64_t T, const int64_t* d_tok_off, const int32_t* d_pos, void* stream) try {
+  if (!ctx) return C4S_ERR_INVALID;
+  c4s::KvArgs a;
+  unsigned grid;
+  if (dtype < C4S_BF16 || dtype > C4S_FP32) return fail(ctx, C4S_ERR_INVALID, "unknown type");
+  const int rc = kv_args(ctx, cache, d_page_table, table_ld, max_pages, B, d_k, d_v, dtype, token_stride, head_stride,
+                         T, d_tok_off, d_pos, a, grid);
+  if (rc || grid == 0) return rc;
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok) return fail(ctx, C4S_ERR_CUDA, "cannot select the context's device");
+  const KvKernel kern = dtype == C4S_BF16 ? read_kernel<__nv_bfloat16>(cache->bits, cache->dtype)
+                        : dtype == C4S_FP16 ? read_kernel<__half>(cache->bits, cache->dtype)
+                                            : read_kernel<float>(cache->bits, cache->dtype);
+  const cudaError_t e = launch(kern, dim3(grid), c4s::KV_NT, 0, stream, a);
+  return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "cache read launch");
+} catch (...) {
+  return C4S_ERR_INVALID;
+}
+
+int64_t c4s_attention_workspace(c4s_ctx* ctx, int32_t B, int32_t q_heads, int32_t head_dim) {
+  if (!ctx || B < 0 || q_heads < 1 || (head_dim != 64 && head_dim != 96 && head_dim != 128)) return C4S_ERR_INVALID;
+  return attn_work_bytes(ctx, head_dim);
+}
+
+int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* d_page_table, int64_t table_ld,
+                        int32_t max_pages, int32_t B, const void* d_q, int32_t dtype, int32_t q_heads,
+                        int64_t q_batch_stride, int64_t q_head_stride, const int32_t* d_len, const int32_t* d_start,
+                        float scale, void* d_out, int64_t out_batch_stride, int64_t out_head_stride, void* d_work,
+                        int64_t work_bytes, void* stream) try {
+  if (!ctx) return C4S_ERR_INVALID;
+  if (B < 0) return fail(ctx, C4S_ERR_INVALID, "B < 0");
+  if (B == 0) return C4S_OK;
+  if (const char* why = bad_cache(cache, d_page_table, table_ld, max_pages, B)) return fail(ctx, C4S_ERR_INVALID, why);
+  if (dtype != C4S_BF16 && dtype != C4S_FP16) return fail(ctx, C4S_ERR_INVALID, "queries are bf16 or fp16");
+  if (cache->bits == 16 && dtype != cache->dtype) return fail(ctx, C4S_ERR_INVALID, "the cache's rows are of another type");
+  if (q_heads < 1 || q_heads % cache->kv_heads) return fail(ctx, C4S_ERR_INVALID, "q_heads must be a multiple of kv_heads");
+  if (!d_q || !d_len || !d_out || !d_work) return fail(ctx, C4S_ERR_INVALID, "null pointer");
+  if (((uintptr_t)d_q & 1) || ((uintptr_t)d_out & 1) || ((uintptr_t)d_work & 15))
+    return fail(ctx, C4S_ERR_INVALID, "misaligned pointer");
+  if (!std::isfinite(scale)) return fail(ctx, C4S_ERR_INVALID, "scale must be finite");
+  if (work_bytes < attn_work_bytes(ctx, cache->head_dim)) return fail(ctx, C4S_ERR_INVALID, "workspace too small");
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok) return fail(ctx, C4S_ERR_CUDA, "cannot select the context's device");
+  const int G = q_heads / cache->kv_heads, NQ = G <= 4 ? 4 : 8;
+  const AttnPick k = dtype == C4S_BF16
+                         ? (NQ == 4 ? attn_pick_dim<__nv_bfloat16, 4>(cache->head_dim, cache->bits, cache->group)
+                                    : attn_pick_dim<__nv_bfloat16, 8>(cache->head_dim, cache->bits, cache->group))
+                         : (NQ == 4 ? attn_pick_dim<__half, 4>(cache->head_dim, cache->bits, cache->group)
+                                    : attn_pick_dim<__half, 8>(cache->head_dim, cache->bits, cache->group));
+  cudaError_t e = cudaFuncSetAttribute(k.main, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "attention kernel attribute");
+  const int ctas = ctx->num_sms * ATT_CTAS;
+  c4s::AttnArgs a;
+  a.c = view(cache);
+  a.table_ld = table_ld;
+  a.max_pages = max_pages;
+  a.qb = q_batch_stride;
+  a.qh = q_head_stride;
+  a.G = G;
+  a.scale = scale * 1.4426950408889634f;           // log2(e): the softmax works in powers of two
+  a.ob = out_batch_stride;
+  a.oh = out_head_stride;
+  a.part_o = static_cast<float*>(d_work);
+  a.part_ml = a.part_o + (size_t)ctas * c4s::ATT_WARPS * 2 * NQ * cache->head_dim;
+  a.errflags = ctx->d_err;
+  for (int b0 = 0; b0 < B; b0 += c4s::ATT_MAXB) {
+    a.B = std::min(c4s::ATT_MAXB, B - b0);
+    a.table = d_page_table + (int64_t)b0 * table_ld;
+    a.q = static_cast<const unsigned short*>(d_q) + (int64_t)b0 * q_batch_stride;
+    a.out = static_cast<unsigned short*>(d_out) + (int64_t)b0 * out_batch_stride;
+    a.len = d_len + b0;
+    a.start = d_start ? d_start + b0 : nullptr;
+    // no more warps than there can be tiles
+    const long long most = (long long)a.B * c4s::kv_tiles(0, (long long)max_pages * cache->page_size, k.tok) *
+                           cache->kv_heads * ((G + NQ - 1) / NQ);
+    const int grid = (int)std::min<long long>(ctas, (most + c4s::ATT_WARPS - 1) / c4s::ATT_WARPS);
+    e = launch(k.main, dim3((unsigned)grid), 32 * c4s::ATT_WARPS, k.smem, stream, a);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "attention launch");
+    e = launch(k.join, dim3((unsigned)(grid * c4s::ATT_WARPS)), 32 * c4s::ATT_WARPS, 0, stream, a, k.tok);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "attention join launch");
+  }
+  return C4S_OK;
+} catch (...) {
+  return C4S_ERR_INVALID;
+}
+
+}  // extern "C"

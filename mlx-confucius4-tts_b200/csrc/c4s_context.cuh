@@ -1,0 +1,94 @@
+// c4s_context.cuh -- the context behind the C ABI and the host helpers that
+// every translation unit of the library shares.
+#pragma once
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_runtime.h>
+
+#include <mutex>
+#include <string>
+#include <vector>
+
+#include "../../include/c4s_sampling.h"
+
+namespace c4s {
+struct RowJob;
+}
+
+struct c4s_ctx {
+  int device = 0;
+  int max_vocab = 0;
+  int num_sms = 0;
+  int scratch_ctas = 0;
+  int scratch_stride = 0;
+  int chunk = 0;                               // rows per split-path launch sequence (<= K_CHUNK)
+  unsigned long long* d_scratch = nullptr;
+  unsigned* d_err = nullptr;
+  unsigned long long* d_counters = nullptr;
+  c4s_row_params* d_default_params = nullptr;  // one zeroed struct (argmax reads no field)
+  int row_occ = 0;                             // resident row-kernel CTAs per SM
+  int list_occ = 0;                            // resident list-kernel CTAs per SM
+  int fused_occ = 0;                           // resident fused-kernel CTAs per SM
+  int fused_small_occ = 0;                     //   and of its small-batch form
+  int fused_mid_occ = 0;                       //   and of its two-per-SM form
+  bool split_dirty = false;                    // a split-path launch sequence stopped early: its
+                                               // queue counters may be stale until cleared
+  c4s::RowJob* d_jobs = nullptr;               // fast path: per-row jobs of one chunk
+  unsigned long long* d_lkeys = nullptr;       //   candidate lists [chunk][LCAP]
+  unsigned long long* d_lsb = nullptr;
+  int* d_defer_rows = nullptr;                 //   rows handed to the general path, then long lists
+  int* d_order = nullptr;                      //   the row kernel's rows by cost class
+  unsigned* d_defer_cnt = nullptr;
+  int debug = 0;
+  bool timing = false;                         // c4s_kernel_timing: events between fast-path launches
+  std::vector<cudaEvent_t> tev;                //   TEV per recorded chunk: before the first kernel, then after
+                                               //   the order, row, list, general and fused kernels
+  std::vector<unsigned char> tev_mask;         //   per recorded chunk: bit k = kernel k ran
+  size_t tev_used = 0;
+  int cached_V = -1;
+  int cached_occ = 0;
+  size_t qg_smem_set = 0;                      // dynamic shared memory allowed for the quantized GEMV
+  std::string last_error;
+};
+
+namespace {
+
+inline int fail(c4s_ctx* ctx, int code, const std::string& msg) {
+  if (ctx) ctx->last_error = msg;
+  return code;
+}
+
+inline int cuda_fail(c4s_ctx* ctx, cudaError_t e, const char* what) {
+  return fail(ctx, C4S_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+// Makes ctx->device current for the lifetime of the guard.
+struct DeviceGuard {
+  int prev = -1;
+  bool ok = true;
+  explicit DeviceGuard(int dev) {
+    if (cudaGetDevice(&prev) != cudaSuccess) { ok = false; return; }
+    if (prev != dev && cudaSetDevice(dev) != cudaSuccess) ok = false;
+  }
+  ~DeviceGuard() {
+    int cur;
+    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+  }
+};
+
+// cuTensorMapEncodeTiled from the driver, through the runtime (no -lcuda).
+inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+}  // namespace

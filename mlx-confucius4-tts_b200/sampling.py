@@ -23,7 +23,7 @@ import threading
 
 import numpy as np
 
-from . import workloads
+from . import block, workloads
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libc4s.so")
@@ -107,6 +107,7 @@ def library() -> C.CDLL:
                 "c4s_head_sample": ([vp, vp, i32, i32, i64, vp, vp, C.c_float, vp, i32, i64, vp, vp, vp, i64,
                                      vp, vp, i64, vp, i32, vp, vp, vp, vp], C.c_int),
             }
+            sig.update(block.signatures())
             for name, (args, res) in sig.items():
                 f = getattr(L, name)
                 f.argtypes = args
@@ -132,7 +133,7 @@ def params_tensor(params: np.ndarray, device) -> "torch.Tensor":
     return torch.from_numpy(raw.copy()).to(device)
 
 
-class SamplingContext:
+class SamplingContext(block.BlockOps):
     """One c4s context (device workspace) bound to a CUDA device.
 
     ``max_rows`` sizes the workspace for batches of up to that many rows per

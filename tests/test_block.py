@@ -1,0 +1,129 @@
+"""The decoder block's operators without a GPU: the index arithmetic of the
+paged cache and of the attention's split compiled for the host, and the
+refusals of the Python and C entry points."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
+import pytest
+
+from conftest import load_c4s
+
+torch = pytest.importorskip("torch")
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_index_arithmetic(tmp_path):
+    exe = tmp_path / "test_kv_index"
+    subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-o", str(exe), os.path.join(HERE, "cpp", "test_kv_index.cpp")],
+                   check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def _cache(bits=16, dtype=torch.bfloat16, pages=4, page=16, heads=2, dim=64, group=64, token_major=False):
+    return load_c4s().KVCache.empty(pages, page, heads, dim, dtype=dtype, bits=bits, group=group,
+                                    token_major=token_major, device="cpu")
+
+
+def test_cache_describes_its_tensors():
+    c = _cache()
+    s = c.struct
+    assert (s.num_pages, s.kv_heads, s.page_size, s.head_dim, s.bits, s.dtype) == (4, 2, 16, 64, 16, 0)
+    assert (s.page_stride, s.head_stride, s.token_stride) == (2 * 16 * 128, 16 * 128, 128)
+    c = _cache(bits=4, dim=128, group=32, token_major=True)
+    s = c.struct
+    assert (s.num_pages, s.kv_heads, s.page_size, s.head_dim, s.bits, s.group) == (4, 2, 16, 128, 4, 32)
+    assert (s.page_stride, s.head_stride, s.token_stride) == (16 * 2 * 64, 64, 2 * 64)
+    assert (s.sb_page_stride, s.sb_head_stride, s.sb_token_stride) == (16 * 2 * 32, 32, 2 * 32)
+
+
+def test_cache_refusals():
+    K = load_c4s().KVCache
+    x = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
+    q = torch.zeros((4, 2, 16, 64), dtype=torch.uint8)
+    sb = torch.zeros((4, 2, 16, 1, 2))
+    with pytest.raises(ValueError):
+        K(x, x.transpose(1, 2).contiguous().transpose(1, 2))         # strides differ
+    with pytest.raises(ValueError):
+        K(x, x, sb, sb)                                              # scales of a 16-bit cache
+    with pytest.raises(TypeError):
+        K(x.float(), x.float())
+    with pytest.raises(ValueError):
+        K(x[..., :32], x[..., :32])                                  # head_dim 32
+    with pytest.raises(ValueError):
+        K(x[..., ::2], x[..., ::2])                                  # rows not contiguous
+    with pytest.raises(ValueError):
+        K(q, q, bits=8)                                              # no scales
+    with pytest.raises(TypeError):
+        K(x, x, sb, sb, bits=8)
+    with pytest.raises(ValueError):
+        K(q, q, sb, sb, bits=5)
+    with pytest.raises(ValueError):
+        K(q, q, sb, sb, bits=4)                                      # a group of 128
+    with pytest.raises(ValueError):
+        K(q, q, sb.expand(4, 2, 16, 3, 2), sb.expand(4, 2, 16, 3, 2), bits=8)
+    with pytest.raises(ValueError):
+        K.empty(4, 16, 2, 96, bits=8, group=64, device="cpu")
+
+
+def test_call_refusals():
+    c4s = load_c4s()
+    b = c4s.block
+    c = _cache()
+    i32 = lambda *n: torch.zeros(n, dtype=torch.int32)
+    table, pos = i32(3, 2), i32(3)
+    kv = torch.zeros((3, 2, 64), dtype=torch.bfloat16)
+    off = torch.zeros(4, dtype=torch.int64)
+    assert b.check_kv(c, table, kv, kv, pos, None, True) == (3, 3, 0)
+    assert b.check_kv(c, table, kv[:2], kv[:2], pos, off, True) == (3, 2, 0)
+    for bad in [lambda: b.check_kv(c, table.long(), kv, kv, pos, None, True),
+                lambda: b.check_kv(c, table, kv.half(), kv.half(), pos, None, True),
+                lambda: b.check_kv(c, table, kv.float(), kv.float(), pos, None, True),
+                lambda: b.check_kv(c, table, kv, kv, pos.long(), None, True),
+                lambda: b.check_kv(c, table, kv, kv, pos, off.int(), True)]:
+        with pytest.raises(TypeError):
+            bad()
+    for bad in [lambda: b.check_kv(c, table[:, :0], kv, kv, pos, None, True),
+                lambda: b.check_kv(c, table.t().contiguous().t(), kv, kv, pos, None, True),
+                lambda: b.check_kv(c, table, kv[:2], kv[:2], pos, None, True),       # two tokens, three sequences
+                lambda: b.check_kv(c, table, kv, kv, pos[:2], None, True),
+                lambda: b.check_kv(c, table, kv, kv, pos, off[:3], True),
+                lambda: b.check_kv(c, table, kv[:, :1], kv[:, :1], pos, None, True),
+                lambda: b.check_kv(c, table, kv.expand(3, 2, 64)[..., :32], kv[..., :32], pos, None, True),
+                lambda: b.check_kv(c, table, kv, kv.float(), pos, None, True),
+                lambda: b.check_kv(c, table, kv[:1].expand(3, 2, 64), kv[:1].expand(3, 2, 64), pos, None, False)]:
+        with pytest.raises(ValueError):
+            bad()
+    q = torch.zeros((3, 4, 64), dtype=torch.bfloat16)
+    assert b.check_attention(q, c, table, pos, None, None) == (3, 4, 0)
+    assert b.check_attention(q.half(), _cache(bits=8), table, pos, pos, None) == (3, 4, 1)
+    for bad in [lambda: b.check_attention(q.half(), c, table, pos, None, None),
+                lambda: b.check_attention(q, c, table, pos.long(), None, None),
+                lambda: b.check_attention(q.float(), _cache(bits=8), table, pos, None, None)]:
+        with pytest.raises(TypeError):
+            bad()
+    for bad in [lambda: b.check_attention(q[:, :3], c, table, pos, None, None),
+                lambda: b.check_attention(q[:2], c, table, pos, None, None),
+                lambda: b.check_attention(q[..., :32], c, table, pos, None, None),
+                lambda: b.check_attention(q, c, table, pos[:2], None, None),
+                lambda: b.check_attention(q, c, table, pos, pos[:1], None),
+                lambda: b.check_attention(q, c, table, pos, None, q[:, :2]),
+                lambda: b.check_attention(q, c, table, pos, None, q.half()),
+                lambda: b.check_attention(q, c, table, pos, None, q[:1].expand(3, 4, 64))]:
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_null_context_is_refused():
+    """The C entries refuse a null context before they look at anything else."""
+    c4s = load_c4s()
+    lib = c4s.library()
+    s = C.byref(_cache().struct)
+    assert lib.c4s_kv_write(None, s, None, 1, 1, 1, None, None, 0, 0, 0, 1, None, None, None) == -1
+    assert lib.c4s_kv_read(None, s, None, 1, 1, 1, None, None, 0, 0, 0, 1, None, None, None) == -1
+    assert lib.c4s_attention_workspace(None, 1, 1, 64) == -1
+    assert lib.c4s_paged_attention(None, s, None, 1, 1, 1, None, 0, 1, 0, 0, None, None, 1.0, None, 0, 0, None, 0,
+                                   None) == -1

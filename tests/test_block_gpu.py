@@ -1,0 +1,485 @@
+"""The decoder block's operators on the GPU against plain fp64 restatements.
+
+Cache: every value read back equals its definition (codes decided in fp64, the
+value scale code + bias to two fp32 roundings); what no token names keeps its
+bits. Attention: fp64 softmax over the values that the cache holds.
+
+Tolerance of the attention, from its arithmetic: the output is rounded once
+(half a step, eps / 2 of its size). Before that, with w = sum_p p |v|:
+scores are fp32 sums of D exact products (D 2^-24 of sum |q k| scale, and one
+rounding of the code's scale and bias each), which moves p by twice that;
+2^x, its argument's rounding (2^-23 |x|) and the sums in blocks of 16 tokens
+(n / 16 + 64 roundings of 2^-23, the accumulator's truncation included) follow;
+P's halves leave 2^-16 (bf16) of it at most.
+"""
+import math
+
+import numpy as np
+import pytest
+
+from conftest import load_c4s
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+BF, FP = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def c4s():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return load_c4s()
+
+
+@pytest.fixture(scope="module")
+def ctx(c4s):
+    return c4s.SamplingContext(max_vocab=64, device=0, max_rows=1)
+
+
+DEV = "cuda:0"
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def new_rows(n, heads, dim, dtype, g):
+    x = torch.randn((n, heads, dim), generator=g, device=DEV) * 0.7
+    x[..., 3::29] *= 8
+    return x.to(dtype)
+
+
+def tables(lens, page, g, spare=3):
+    need = [max(0, -(-n // page)) for n in lens]
+    perm = torch.randperm(sum(need) + spare, generator=g, device=DEV).to(torch.int32)
+    t = torch.full((len(lens), max(1, max(need))), -1, dtype=torch.int32, device=DEV)
+    k = 0
+    for b, n in enumerate(need):
+        t[b, :n] = perm[k:k + n]
+        k += n
+    return t, sum(need) + spare
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def quantised(x, bits, group):
+    """fp64 values, and the fp32 (scale, bias) pairs, of rows x."""
+    n = 2 ** bits - 1
+    g = x.double().unflatten(-1, (-1, group))
+    lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+    code = torch.where(hi > lo, torch.round((g - lo) * n / (hi - lo)), 0.0)
+    scale = ((hi - lo) / n).float()
+    return (code * scale.double() + lo).flatten(-2), torch.cat([scale, lo.float()], -1), code.flatten(-2)
+
+
+def dense(cache, table, lens):
+    """fp64 (k, v) per sequence [n, heads, dim] of what a cache holds."""
+    out = []
+    for x, sb in ((cache.k, cache.k_sb), (cache.v, cache.v_sb)):
+        per = []
+        for b, n in enumerate(lens):
+            p = torch.arange(max(0, n), device=DEV)
+            page, slot = table[b].long()[p // cache.page_size], p % cache.page_size
+            r = x[page, :, slot]
+            if sb is not None:
+                if cache.bits == 4:
+                    r = torch.stack([r & 15, r >> 4], -1).flatten(-2)
+                pr = sb[page, :, slot].double()
+                r = (r.double().unflatten(-1, (pr.shape[-2], -1)) * pr[..., :1] + pr[..., 1:]).flatten(-2)
+            per.append(r.double())
+        out.append(per)
+    return out
+
+
+CACHES = [(16, BF, 64), (16, FP, 64), (8, BF, 64), (8, FP, 32), (4, BF, 64), (4, FP, 32)]
+
+
+@pytest.mark.parametrize("bits,dtype,group", CACHES)
+@pytest.mark.parametrize("dim,heads,page,token_major,lens,before", [
+    (64, 20, 16, False, [1] * 5, [0, 15, 16, 200, 31]),              # a decode step, at page borders
+    (128, 3, 25, True, [7, 0, 33, 1, 300], [0, 3, 24, 25, 1]),       # ragged, an empty sequence
+    (96, 2, 1, False, [40, 9], [0, 5]),                              # pages of one slot
+    (64, 1, 100, True, [257], [0]),
+])
+def test_cache_written_and_read(ctx, c4s, bits, dtype, group, dim, heads, page, token_major, lens, before):
+    if dim % group and bits != 16:
+        group = 32
+    g = gen(bits + dim + page)
+    table, pages = tables([a + n for a, n in zip(before, lens)], page, g)
+    cache = c4s.KVCache.empty(pages, page, heads, dim, dtype=dtype, bits=bits, group=group, token_major=token_major,
+                              device=DEV)
+    for x in (cache.k, cache.v, cache.k_sb, cache.v_sb):
+        if x is not None:
+            x.fill_(7)
+    kept = [None if x is None else x.clone() for x in (cache.k, cache.v, cache.k_sb, cache.v_sb)]
+    T = sum(lens)
+    qkv = torch.empty((T, 3, heads, dim), dtype=dtype, device=DEV)   # rows of a fused projection
+    qkv[:, 1], qkv[:, 2] = new_rows(T, heads, dim, dtype, g), new_rows(T, heads, dim, dtype, g)
+    qkv[0, 1, 0] = 0.25                                              # constant groups
+    k, v = qkv[:, 1], qkv[:, 2]
+    off = torch.tensor([0] + list(np.cumsum(lens)), dtype=torch.int64, device=DEV)
+    step = all(n == 1 for n in lens)
+    ctx.kv_write(cache, table, k, v, i32(before), tok_off=None if step else off)
+    rk, rv = ctx.kv_read(cache, table, i32(before), tok_off=None if step else off, total=T, dtype=torch.float32)
+    seq = torch.repeat_interleave(torch.arange(len(lens), device=DEV), torch.tensor(lens, device=DEV))
+    at = torch.arange(T, device=DEV) - off[seq] + i32(before)[seq]
+    pg, sl = table[seq, at // page].long(), at % page
+    for x, new, got, pool, sb, k0, s0 in ((cache.k, k, rk, cache.k, cache.k_sb, kept[0], kept[2]),
+                                          (cache.v, v, rv, cache.v, cache.v_sb, kept[1], kept[3])):
+        if bits == 16:
+            assert torch.equal(got, new.float())
+            k0[pg, :, sl] = new
+        else:
+            want, pairs, code = quantised(new, bits, group)
+            size = (code.unflatten(-1, (-1, group)) * pairs[..., :1].double()).abs().flatten(-2) + want.abs()
+            # the fp32 scale may be one step off the fp64 one, and the value is rounded once
+            assert torch.all((got.double() - want).abs() <= size * 2.0 ** -22)
+            c = code.to(torch.uint8)
+            k0[pg, :, sl] = c if bits == 8 else c[..., 0::2] | (c[..., 1::2] << 4)
+            s0[pg, :, sl] = sb[pg, :, sl]
+            assert torch.equal(sb, s0)
+        assert torch.equal(pool, k0)                                 # codes, and nothing else touched
+    for dt in (BF, FP):
+        rk2, rv2 = ctx.kv_read(cache, table, i32(before), tok_off=None if step else off, total=T, dtype=dt)
+        assert torch.equal(rk2, rk.to(dt)) and torch.equal(rv2, rv.to(dt))
+    assert ctx.status()[0] == 0
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_cache_codes_at_ties_and_odd_groups(ctx, c4s, bits):
+    """Values on a grid make exact ties; NaN and infinity spoil their own group only; ranges past fp32 and near its
+    smallest numbers keep their codes."""
+    n = 2 ** bits - 1
+    x = torch.zeros((6, 1, 128), device=DEV)
+    r = torch.arange(64, device=DEV).float()
+    x[0, 0, :64] = r % (2 * n + 1)                                   # span 2 n: every odd value is a tie
+    x[0, 0, 63] = 2 * n
+    x[0, 0, 62] = 0
+    x[1, 0, :64] = r / 63
+    x[1, 0, 64:] = -r
+    x[2, 0, 5] = float("nan")
+    x[2, 0, 64:] = r
+    x[3, 0, 70] = float("-inf")
+    x[4, 0, :64] = (r - 31) * 1e37
+    x[4, 0, 3] = 3e38
+    x[4, 0, 4] = -3e38
+    x[5, 0, :64] = r * 1e-39
+    x = x.to(BF)
+    cache = c4s.KVCache.empty(2, 8, 1, 128, bits=bits, group=64, device=DEV)
+    table, pos = i32([[1]]), i32([0])
+    off = torch.tensor([0, 6], dtype=torch.int64, device=DEV)
+    ctx.kv_write(cache, table, x, x.clone(), pos, tok_off=off)
+    got, gv = ctx.kv_read(cache, table, pos, tok_off=off, total=6, dtype=torch.float32)
+    want, pairs, code = quantised(x, bits, 64)
+    q = cache.k[1, 0, :6]
+    q = q if bits == 8 else torch.stack([q & 15, q >> 4], -1).flatten(-2)
+    fine = torch.ones((6, 128), dtype=torch.bool, device=DEV)
+    fine[2, :64] = False
+    fine[3, 64:] = False
+    assert torch.equal(q.double()[fine], code[:, 0][fine])
+    assert torch.isnan(got[:, 0][~fine]).all() and torch.isfinite(got[:, 0][fine]).all()
+    rows = [0, 1, 2, 3]
+    tol = (want.abs() + pairs[..., :1].double().repeat_interleave(64, -2).flatten(-2) * n) * 2.0 ** -21
+    ok = fine & (torch.arange(6, device=DEV) < 4)[:, None]
+    assert torch.all((got[:, 0].double() - want[:, 0]).abs()[ok] <= tol[:, 0][ok]), rows
+    assert torch.equal(got.isnan(), gv.isnan())
+
+
+def test_cache_skips_and_bad_pages(ctx, c4s):
+    """Sequences at a negative position and tokens behind the last are left alone; a position without a page is left
+    out, reads as zero and is reported."""
+    g = gen(3)
+    cache = c4s.KVCache.empty(4, 4, 2, 64, dtype=BF, device=DEV)
+    table = i32([[0, 1], [2, -1], [3, 9]])
+    off = torch.tensor([0, 3, 8, 12], dtype=torch.int64, device=DEV)
+    k, v = new_rows(15, 2, 64, BF, g), new_rows(15, 2, 64, BF, g)
+    ctx.kv_write(cache, table, k, v, i32([-1, 0, 2]), tok_off=off)
+    err, _ = ctx.status(reset=True)
+    assert err == 16
+    want = torch.zeros_like(cache.k)
+    want[2, :, :4] = k[3:7].transpose(0, 1)
+    want[3, :, 2:4] = k[8:10].transpose(0, 1)
+    assert torch.equal(cache.k, want)
+    ko, vo = torch.full((15, 2, 64), 5.0, device=DEV), torch.full((15, 2, 64), 5.0, device=DEV)
+    ctx.kv_read(cache, table, i32([-1, 0, 2]), tok_off=off, k_out=ko, v_out=vo)
+    err, _ = ctx.status(reset=True)
+    assert err == 16
+    full = torch.full((15, 2, 64), 5.0, device=DEV)
+    full[3:12] = 0
+    full[3:7], full[8:10] = k[3:7].float(), k[8:10].float()
+    assert torch.equal(ko, full)
+    # nothing to do
+    ctx.kv_write(cache, table[:0], k[:0], v[:0], i32([]))
+    ctx.kv_write(cache, table, k[:0], v[:0], i32([0, 0, 0]), tok_off=torch.zeros(4, dtype=torch.int64, device=DEV))
+    assert torch.equal(cache.k, want) and ctx.status()[0] == 0
+
+
+def test_cache_rows_not_aligned(ctx, c4s):
+    """Source rows that start on no 16-byte border."""
+    g = gen(4)
+    cache = c4s.KVCache.empty(3, 8, 2, 64, dtype=BF, bits=8, device=DEV)
+    flat = torch.randn(2 * 5 * 131 + 1, generator=g, device=DEV).to(BF)
+    k = flat[1:1 + 5 * 2 * 131].view(5, 2, 131)[..., :64]
+    table, off = i32([[2]]), torch.tensor([0, 5], dtype=torch.int64, device=DEV)
+    ctx.kv_write(cache, table, k, k, i32([0]), tok_off=off)
+    out = torch.full((5, 2, 67), 9.0, device=DEV)
+    ctx.kv_read(cache, table, i32([0]), tok_off=off, k_out=out[..., 1:65], v_out=out.clone()[..., 1:65])
+    want, _, _ = quantised(k, 8, 64)
+    assert torch.all((out[..., 1:65].double() - want).abs() <= 2.0 ** -20 * (1 + want.abs()))
+    assert torch.all(out[..., 0] == 9) and torch.all(out[..., 65:] == 9)
+
+
+def filled(c4s, lens, heads, dim, page, dtype, bits, group, g, token_major=False, nan=True):
+    """A cache with every slot filled; what no sequence sees is NaN."""
+    table, pages = tables(lens, page, g)
+    cache = c4s.KVCache.empty(pages, page, heads, dim, dtype=dtype, bits=bits, group=group, token_major=token_major,
+                              device=DEV)
+    for x, sb in ((cache.k, cache.k_sb), (cache.v, cache.v_sb)):
+        rows = new_rows(pages * page, heads, dim, dtype, g)
+        if bits == 16:
+            x.copy_(rows.view(pages, page, heads, dim).transpose(1, 2))
+        else:
+            _, pairs, code = quantised(rows, bits, group)
+            c = code.to(torch.uint8)
+            c = c if bits == 8 else c[..., 0::2] | (c[..., 1::2] << 4)
+            x.copy_(c.view(pages, page, heads, -1).transpose(1, 2))
+            sb.copy_(pairs.view(pages, page, heads, -1, 2).transpose(1, 2))
+        if nan:
+            seen = torch.zeros((pages, page), dtype=torch.bool, device=DEV)
+            for b, n in enumerate(lens):
+                p = torch.arange(max(0, n), device=DEV)
+                seen[table[b].long()[p // page], p % page] = True
+            (x if bits == 16 else sb).transpose(1, 2)[~seen] = float("nan")
+    return cache, table
+
+
+def check_attention(ctx, c4s, q, cache, table, lens, start, scale, out):
+    k, v = dense(cache, table, lens)
+    G = q.shape[1] // cache.kv_heads
+    half = torch.finfo(q.dtype).eps / 2
+    for b, n in enumerate(lens):
+        a = 0 if start is None else max(0, start[b])
+        if n <= a:
+            assert torch.all(out[b] == 0), b
+            continue
+        kb = k[b][a:].repeat_interleave(G, 1)                        # [n, q_heads, dim]
+        vb = v[b][a:].repeat_interleave(G, 1)
+        qb = q[b].double()
+        s = torch.einsum("hd,nhd->hn", qb, kb) * scale
+        size = torch.einsum("hd,nhd->hn", qb.abs(), kb.abs()).amax(1) * abs(scale)
+        if cache.bits != 16:                                         # codes: code scale and bias cancel
+            size = size + 2 * (qb.abs().sum(1) * kb.abs().amax((0, 2)) * abs(scale))
+        p = torch.softmax(s, 1)
+        ref = torch.einsum("hn,nhd->hd", p, vb)
+        w = torch.einsum("hn,nhd->hd", p, vb.abs())
+        if cache.bits != 16:
+            w = w + vb.abs().amax((0, 2))[:, None] * 2
+        steps = (n - a) / 16 + 64
+        rel = 2 * ((cache.head_dim + 8) * 2.0 ** -24 * size + 2.0 ** -23 * s.abs().amax(1)) + 2.0 ** -16 + \
+            steps * 2.0 ** -23
+        err = (out[b].double() - ref).abs()
+        tiny = torch.finfo(q.dtype).smallest_normal * half
+        bound = ref.abs() * half * 1.001 + w * rel[:, None] * (1 + half) + tiny
+        assert torch.all(err <= bound), (b, float((err / bound).max()))
+
+
+ATTENTION = [
+    # heads, shared, dim, page, lens, start
+    (20, 1, 64, 16, [1, 0, 17, 300, 33, 64, 5], None),
+    (2, 3, 64, 25, [70, 31, 1, 0, 500], [60, 31, 0, 0, -4]),         # windows, one of them empty
+    (4, 4, 128, 32, [129, 1000], None),
+    (1, 5, 96, 1, [77, 130], None),                                  # pages of one slot, five heads
+    (2, 8, 128, 128, [1500], None),
+    (1, 16, 64, 100, [2, 999], [1, 990]),                            # two passes over a key head
+    (3, 1, 96, 8, [15, 16, 17], None),
+]
+
+
+@pytest.mark.parametrize("bits,dtype,group", CACHES)
+@pytest.mark.parametrize("heads,shared,dim,page,lens,start", ATTENTION)
+def test_attention(ctx, c4s, bits, dtype, group, heads, shared, dim, page, lens, start):
+    if dim % group:
+        group = 32
+    g = gen(heads * 100 + dim + bits)
+    cache, table = filled(c4s, lens, heads, dim, page, dtype, bits, group, g, token_major=page % 2 == 0)
+    q = (torch.randn((len(lens), heads * shared, dim), generator=g, device=DEV) * 0.8).to(dtype)
+    scale = 1 / math.sqrt(dim)
+    out = ctx.paged_attention(q, cache, table, i32(lens), start=None if start is None else i32(start))
+    check_attention(ctx, c4s, q, cache, table, lens, start, scale, out)
+    assert ctx.status()[0] == 0
+
+
+@pytest.mark.parametrize("bits,dtype", [(16, BF), (16, FP), (8, BF), (4, FP)])
+def test_attention_joins_one_long_sequence(ctx, c4s, bits, dtype):
+    """One sequence over every warp of the machine, and sharp and flat softmaxes."""
+    lens = [70001]
+    g = gen(9)
+    cache, table = filled(c4s, lens, 1, 64, 64, dtype, bits, 64, g)
+    work = ctx.attention_workspace(1, 2, 64)
+    for gain in (0.0, 0.3, 6.0):
+        q = (torch.randn((1, 2, 64), generator=g, device=DEV) * gain).to(dtype)
+        out = ctx.paged_attention(q, cache, table, i32(lens), work=work)
+        check_attention(ctx, c4s, q, cache, table, lens, None, 0.125, out)
+
+
+def test_attention_many_sequences(ctx, c4s):
+    """More sequences than one launch takes, most of them short, pages shared between them."""
+    g = gen(10)
+    B, base = 1100, [200, 40, 0, 3]
+    cache, t4 = filled(c4s, base, 2, 64, 16, BF, 16, 64, g)
+    lens = [base[b % 4] for b in range(B)]
+    table = t4.repeat(B // 4, 1)
+    q = torch.randn((B, 2, 64), generator=g, device=DEV).to(BF)
+    out = ctx.paged_attention(q, cache, table, i32(lens))
+    check_attention(ctx, c4s, q, cache, table, lens, None, 0.125, out)
+
+
+def test_attention_strides_scale_and_out(ctx, c4s):
+    """Queries as a slice of a fused projection, at odd offsets; outputs into a slice, the rest left as it was."""
+    g = gen(11)
+    lens = [40, 90, 7]
+    cache, table = filled(c4s, lens, 4, 64, 16, FP, 16, 64, g)
+    wide = torch.randn((3, 4 * 67 + 5), generator=g, device=DEV).to(FP)
+    q = wide[:, 1:1 + 4 * 67].unflatten(1, (4, 67))[..., 2:66]
+    buf = torch.full((3, 6, 70), 3.0, device=DEV).to(FP)
+    out = buf[:, 1:5, 3:67]
+    wtable = torch.full((3, table.shape[1] + 4), 12345, dtype=torch.int32, device=DEV)
+    wtable[:, :table.shape[1]] = table
+    got = ctx.paged_attention(q, cache, wtable[:, :table.shape[1]], i32(lens), scale=0.31, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    check_attention(ctx, c4s, q, cache, table, lens, None, 0.31, out)
+    assert torch.all(buf[:, 0] == 3) and torch.all(buf[:, 5] == 3) and torch.all(buf[..., :3] == 3)
+    assert torch.all(buf[:, 1:5, 67:] == 3)
+
+
+def test_attention_non_finite(ctx, c4s):
+    """A NaN or infinite key spoils its own sequence and head, nothing else; a NaN value likewise."""
+    g = gen(12)
+    lens = [50, 50, 50]
+    cache, table = filled(c4s, lens, 2, 64, 16, BF, 16, 64, g)
+    q = torch.randn((3, 2, 64), generator=g, device=DEV).to(BF)
+    clean = ctx.paged_attention(q, cache, table, i32(lens))
+    cache.k[table[0, 1].long(), 0, 3, 7] = float("nan")
+    cache.v[table[1, 2].long(), 1, 0, 9] = float("nan")
+    out = ctx.paged_attention(q, cache, table, i32(lens))
+    assert torch.isnan(out[0, 0]).all() and torch.equal(out[0, 1], clean[0, 1])
+    assert torch.isnan(out[1, 1, 9]) and not torch.isnan(out[1, 1, :9]).any() and torch.equal(out[1, 0], clean[1, 0])
+    assert torch.equal(out[2], clean[2])
+    # behind a window nothing counts
+    out = ctx.paged_attention(q, cache, table, i32(lens), start=i32([20, 0, 0]))
+    assert not torch.isnan(out[0]).any()
+
+
+def test_attention_bad_pages(ctx, c4s):
+    """Positions without a page are left out and reported; the rest is attended to."""
+    g = gen(13)
+    lens = [64, 64]
+    cache, table = filled(c4s, lens, 1, 64, 16, BF, 16, 64, g, nan=False)
+    q = torch.randn((2, 1, 64), generator=g, device=DEV).to(BF)
+    bad = table.clone()
+    bad[0, 1], bad[0, 3] = -1, 1 << 30
+    out = ctx.paged_attention(q, cache, bad, i32([64, 1 << 30]))      # the second: past the table
+    err, _ = ctx.status(reset=True)
+    assert err == 16
+    k, v = dense(cache, table, lens)
+    keep = torch.tensor([i // 16 in (0, 2) for i in range(64)], device=DEV)
+    p = torch.softmax(q[0, 0].double() @ k[0][keep, 0].T / 8, 0)
+    assert (out[0, 0].double() - p @ v[0][keep, 0]).abs().max() < 0.02
+    p = torch.softmax(q[1, 0].double() @ k[1][:, 0].T / 8, 0)
+    assert (out[1, 0].double() - p @ v[1][:, 0]).abs().max() < 0.02
+
+
+def test_attention_repeats_and_graphs(ctx, c4s):
+    """The same call gives the same bits; two graphs with workspaces of their own, replayed on two streams while
+    lengths grow in place, give what the eager calls give."""
+    g = gen(14)
+    lens = [400, 33, 0, 1200]
+    cache, table = filled(c4s, [n + 8 for n in lens], 4, 64, 16, BF, 8, 64, g, nan=False)
+    q = torch.randn((4, 4, 64), generator=g, device=DEV).to(BF)
+    n = i32(lens)
+    a = ctx.paged_attention(q, cache, table, n)
+    for _ in range(3):
+        assert torch.equal(a, ctx.paged_attention(q, cache, table, n))
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        st = torch.cuda.Stream()
+        work = ctx.attention_workspace(4, 4, 64)
+        out = torch.empty_like(q)
+        st.wait_stream(torch.cuda.current_stream())
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=st):
+            ctx.paged_attention(q, cache, table, n, out=out, work=work)
+        graphs.append((st, gr, out, work))
+    for step in range(8):
+        torch.cuda.synchronize()
+        want = ctx.paged_attention(q, cache, table, n)
+        torch.cuda.synchronize()
+        for st, gr, out, _ in graphs:
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        for _, _, out, _ in graphs:
+            assert torch.equal(out, want), step
+        n += 1
+
+
+def test_other_stream(ctx, c4s):
+    """Calls on a stream that is not the current one, outputs allocated there."""
+    g = gen(15)
+    lens = [100, 3]
+    cache, table = filled(c4s, lens, 2, 64, 16, BF, 16, 64, g, nan=False)
+    q = torch.randn((2, 2, 64), generator=g, device=DEV).to(BF)
+    n = i32(lens)
+    want = ctx.paged_attention(q, cache, table, n)
+    wk, wv = ctx.kv_read(cache, table, n - 1, dtype=torch.float32)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    out = ctx.paged_attention(q, cache, table, n, stream=st)
+    n1 = n - 1
+    st.wait_stream(torch.cuda.current_stream())
+    rk, rv = ctx.kv_read(cache, table, n1, dtype=torch.float32, stream=st)
+    st.synchronize()
+    assert torch.equal(out, want) and torch.equal(rk, wk) and torch.equal(rv, wv)
+
+
+def test_far_pages(ctx, c4s):
+    """Rows more than 2^32 bytes into the cache."""
+    page, heads, dim = 64, 8, 128
+    pages = (1 << 32) // (page * heads * dim * 2) + 50
+    k = torch.empty((pages, heads, page, dim), dtype=BF, device=DEV)
+    v = torch.empty_like(k)
+    cache = c4s.KVCache(k, v)
+    g = gen(16)
+    table = i32([[pages - 1, 0, pages - 7]])
+    x, y = new_rows(150, heads, dim, BF, g), new_rows(150, heads, dim, BF, g)
+    off = torch.tensor([0, 150], dtype=torch.int64, device=DEV)
+    ctx.kv_write(cache, table, x, y, i32([0]), tok_off=off)
+    assert torch.equal(k[pages - 1], x[:64].transpose(0, 1)) and torch.equal(v[pages - 7, :, :22], y[128:].transpose(0, 1))
+    rk, rv = ctx.kv_read(cache, table, i32([0]), tok_off=off, total=150)
+    assert torch.equal(rk, x) and torch.equal(rv, y)
+    q = torch.randn((1, heads, dim), generator=g, device=DEV).to(BF)
+    out = ctx.paged_attention(q, cache, table, i32([150]))
+    check_attention(ctx, c4s, q, cache, table, [150], None, dim ** -0.5, out)
+
+
+def test_c_refusals(ctx, c4s):
+    """What only the C entries see: alignment, workspace, scale."""
+    lib = ctx.lib
+    cache, table = filled(c4s, [20], 2, 64, 16, BF, 16, 64, gen(17), nan=False)
+    q = torch.zeros((1, 2, 64), dtype=BF, device=DEV)
+    with pytest.raises(c4s.C4SError):
+        ctx.paged_attention(q, cache, table, i32([20]), work=torch.zeros(64, dtype=torch.uint8, device=DEV))
+    with pytest.raises(c4s.C4SError):
+        ctx.paged_attention(q, cache, table, i32([20]), scale=float("nan"))
+    odd = torch.zeros((4, 2, 16, 72), dtype=BF, device=DEV)[..., 4:68]
+    with pytest.raises(c4s.C4SError):
+        ctx.paged_attention(q, c4s.KVCache(odd, odd), table, i32([20]))
+    with pytest.raises(ValueError):
+        ctx.paged_attention(q.cpu(), cache, table, i32([20]))
+    assert lib.c4s_attention_workspace(ctx._h, 1, 2, 80) == -1
+    assert ctx.status()[0] == 0
