@@ -301,6 +301,36 @@ int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* 
                         float scale, void* d_out, int64_t out_batch_stride, int64_t out_head_stride, void* d_work,
                         int64_t work_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The linear layer of the GPT-2 blocks, with what surrounds it in one call:
+ *   out = act(LN(x) W^T + b) + residual
+ * (nn.cpp:11-16 linear, nn.cpp:73-83 layer_norm; the projections, the MLP's
+ * GELU and the residual adds of gpt2.cpp's blocks).
+ *   d_x       [M, ld_x] bf16 or fp16 (dtype), K elements a row
+ *   d_norm    [M, K] of dtype, 16-byte aligned: caller-owned workspace of the
+ *             normalised rows (rounded to dtype, the product's operand;
+ *             contents undefined afterwards), with d_gamma, d_beta fp32 [K] or
+ *             NULL (1, 0) and eps; NULL skips the LayerNorm
+ *   d_weight  [N, ld_weight] of dtype (out x in)
+ *   d_bias    fp32 [N] or NULL;  act: C4S_ACT_*
+ *   d_residual  [M, ld_residual] of out_dtype or NULL; may be d_out itself
+ *   d_out     [M, ld_out] of out_dtype: dtype or fp32; not x, not the weight
+ * fp32 accumulation, bias, activation and residual; one rounding at the end.
+ * K a multiple of 8 (with the LayerNorm at most 8192); x (without the
+ * LayerNorm) and the weight 16-byte aligned with strides of whole 16 bytes.
+ * Any M >= 0, N >= 1.                                                       */
+typedef enum c4s_act {
+  C4S_ACT_NONE = 0,
+  C4S_ACT_GELU = 1,      /* 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))): GPT-2's */
+  C4S_ACT_GELU_ERF = 2,  /* 0.5 x (1 + erf(x / sqrt 2)) */
+  C4S_ACT_SILU = 3,
+  C4S_ACT_RELU = 4
+} c4s_act;
+int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t K, int64_t ld_x, const float* d_gamma,
+               const float* d_beta, float eps, void* d_norm, const void* d_weight, int32_t N, int64_t ld_weight,
+               const float* d_bias, int32_t act, const void* d_residual, int64_t ld_residual, void* d_out,
+               int32_t out_dtype, int64_t ld_out, void* stream);
+
 /* Apply the processors selected by `stages` (C4S_STAGE_* bits) in place to B
  * rows of d_logits, in the reference order, ignoring params.greedy.
  * Replaces the in-place processors of sampling.cpp:14-71 / t2s.h:83-88:

@@ -17,6 +17,7 @@ import math
 
 BF16, FP16, FP32 = 0, 1, 2
 HEAD_DIMS = (64, 96, 128)
+ACTIVATIONS = {"none": 0, "gelu": 1, "gelu_erf": 2, "silu": 3, "relu": 4}
 
 
 class _CacheStruct(C.Structure):
@@ -32,6 +33,8 @@ def signatures():
     vp, i32, i64, f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
     kv = [vp, C.POINTER(_CacheStruct), vp, i64, i32, i32, vp, vp, i32, i64, i64, i64, vp, vp, vp]
     return {
+        "c4s_linear": ([vp, vp, i32, i32, i32, i64, vp, vp, f32, vp, vp, i32, i64, vp, i32, vp, i64, vp, i32, i64, vp],
+                       C.c_int),
         "c4s_kv_write": (kv, C.c_int),
         "c4s_kv_read": (kv, C.c_int),
         "c4s_attention_workspace": ([vp, i32, i32, i32], C.c_int64),
@@ -213,6 +216,43 @@ def check_attention(q, cache: KVCache, page_table, lens, start, out):
     return B, q.shape[1], kind
 
 
+def _matrix(t, what: str, shape):
+    if t.dim() != 2 or tuple(t.shape) != tuple(shape) or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what} must be {tuple(shape)} with contiguous rows")
+
+
+def check_linear(x, weight, bias, act, residual, gamma, beta, out, out_dtype):
+    """Refuses what c4s_linear cannot take; returns (M, K, N, c4s_dtype of x, of out, torch type of out)."""
+    torch = _torch()
+    if x.dim() != 2 or weight.dim() != 2:
+        raise ValueError("x must be [M, K] and weight [N, K]")
+    M, K = x.shape
+    N = weight.shape[0]
+    _matrix(x, "x", (M, K))
+    _matrix(weight, "weight", (N, K))
+    kind = _type(x, "x")
+    if _type(weight, "weight") != kind:
+        raise TypeError("x and weight must be of one type")
+    if act not in ACTIVATIONS:
+        raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}")
+    if out_dtype is None:
+        out_dtype = x.dtype if out is None else out.dtype
+    okind = FP32 if out_dtype == torch.float32 else kind
+    if out_dtype != torch.float32 and out_dtype != x.dtype:
+        raise TypeError("out is of x's type or fp32")
+    for name, t, n in (("bias", bias, N), ("gamma", gamma, K), ("beta", beta, K)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (n,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous fp32 [{n}]")
+    for name, t in (("residual", residual), ("out", out)):
+        if t is not None:
+            if t.dtype != out_dtype:
+                raise TypeError(f"{name} must be {out_dtype}")
+            _matrix(t, name, (M, N))
+    if M > 1 and out is not None and out.stride(0) < N:
+        raise ValueError("the rows of out must not overlap")
+    return M, K, N, kind, okind, out_dtype
+
+
 class BlockOps:
     """The block's operators of a context (SamplingContext)."""
 
@@ -290,4 +330,33 @@ class BlockOps:
             None if start is None else start.data_ptr(), scale, out.data_ptr(), out.stride(0), out.stride(1),
             work.data_ptr(), work.numel() * work.element_size(), self._stream(stream))
         self._check(rc, "c4s_paged_attention")
+        return out
+
+    def linear(self, x, weight, bias=None, act: str = "none", residual=None, layer_norm: bool = False, gamma=None,
+               beta=None, eps: float = 1e-5, norm_out=None, out=None, out_dtype=None, stream=None):
+        """act(LN(x) weight^T + bias) + residual (c4s_linear): x [M, K] and
+        weight [N, K] bf16 or fp16 -> out [M, N] of x's type or fp32. bias,
+        gamma, beta fp32; act one of ACTIVATIONS; residual of out's type (it may
+        be out); layer_norm=False skips the LayerNorm; norm_out: [M, K] workspace
+        of the normalised rows."""
+        torch = _torch()
+        M, K, N, kind, okind, out_dtype = check_linear(x, weight, bias, act, residual, gamma, beta, out, out_dtype)
+        _on(self.device, x=x, weight=weight, bias=bias, residual=residual, gamma=gamma, beta=beta, out=out,
+            norm_out=norm_out)
+        if norm_out is not None:
+            _matrix(norm_out, "norm_out", (M, K))
+            if norm_out.dtype != x.dtype or not norm_out.is_contiguous():
+                raise ValueError("norm_out must be contiguous, of x's type")
+        with self._allocating(stream):
+            if out is None:
+                out = torch.empty((M, N), dtype=out_dtype, device=self.device)
+            if layer_norm and norm_out is None:
+                norm_out = torch.empty((M, K), dtype=x.dtype, device=self.device)
+        rc = self.lib.c4s_linear(
+            self._h, x.data_ptr(), kind, M, K, x.stride(0), None if gamma is None else gamma.data_ptr(),
+            None if beta is None else beta.data_ptr(), eps, norm_out.data_ptr() if layer_norm else None,
+            weight.data_ptr(), N, weight.stride(0), None if bias is None else bias.data_ptr(), ACTIVATIONS[act],
+            None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0),
+            out.data_ptr(), okind, out.stride(0), self._stream(stream))
+        self._check(rc, "c4s_linear")
         return out

@@ -1,5 +1,6 @@
 // c4s_block.cu -- C ABI of the decoder block's operators: the paged key-value
-// cache (c4s_kv.cuh) and the attention over it (c4s_attn.cuh).
+// cache (c4s_kv.cuh), the attention over it (c4s_attn.cuh) and the linear
+// layer (c4s_linear.cuh).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -13,6 +14,7 @@
 #include "c4s_kvidx.cuh"
 #include "c4s_kv.cuh"
 #include "c4s_attn.cuh"
+#include "c4s_linear.cuh"
 
 namespace {
 
@@ -145,6 +147,43 @@ template <typename T, int NQ> AttnPick attn_pick_dim(int dim, int bits, int grou
                    : dim == 96 ? attn_pick_rows<T, 96, NQ>(bits, group) : attn_pick_rows<T, 128, NQ>(bits, group);
 }
 
+// 2-D tensor map of `outer` rows of `inner` 16-bit elements read in boxes of
+// 64 x `box` with the 128-byte swizzle; what lies outside reads as zeros.
+bool encode_rows(CUtensorMap* m, int dtype, const void* base, long long inner, long long outer, long long pitch_bytes,
+                 int box) {
+  const PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+  cuuint64_t strides[1] = {(cuuint64_t)pitch_bytes};
+  cuuint32_t bx[2] = {(cuuint32_t)c4s::LN_BK, (cuuint32_t)box};
+  cuuint32_t es[2] = {1, 1};
+  return enc(m, dtype == C4S_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+             const_cast<void*>(base), dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+using TileKernel = void (*)(const CUtensorMap, const CUtensorMap, c4s::LinArgs, int);
+struct TilePick {
+  TileKernel kern;
+  size_t smem;
+};
+template <typename TI, typename TO> TilePick tile_pick(int bn) {
+  return bn == 64 ? TilePick{c4s::lin_tile_kernel<TI, TO, 64>, c4s::LinCfg<64>::SMEM}
+                  : TilePick{c4s::lin_tile_kernel<TI, TO, 128>, c4s::LinCfg<128>::SMEM};
+}
+
+template <typename T>
+cudaError_t launch_norm(const void* x, int M, int K, int64_t ldx, const float* gamma, const float* beta, float eps,
+                        void* y, void* stream) {
+  const bool vec = ((uintptr_t)x & 15) == 0 && (ldx & 7) == 0;
+  const int vpt = (K / 8 + c4s::LNORM_NT - 1) / c4s::LNORM_NT;
+  auto kern = vpt <= 1 ? c4s::lin_norm_kernel<T, 1>
+              : vpt <= 2 ? c4s::lin_norm_kernel<T, 2>
+              : vpt <= 4 ? c4s::lin_norm_kernel<T, 4> : c4s::lin_norm_kernel<T, 8>;
+  return launch(kern, dim3((unsigned)M), c4s::LNORM_NT, 0, stream, (const T*)x, (long long)ldx, K, vec, gamma, beta,
+                eps, (T*)y);
+}
+
 constexpr int ATT_CTAS = 2;                        // per SM: what their shared memory is sized for
 
 int64_t attn_work_bytes(const c4s_ctx* ctx, int dim) {
@@ -260,6 +299,92 @@ int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* 
     if (e != cudaSuccess) return cuda_fail(ctx, e, "attention join launch");
   }
   return C4S_OK;
+} catch (...) {
+  return C4S_ERR_INVALID;
+}
+
+int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t K, int64_t ld_x, const float* d_gamma,
+               const float* d_beta, float eps, void* d_norm, const void* d_weight, int32_t N, int64_t ld_weight,
+               const float* d_bias, int32_t act, const void* d_residual, int64_t ld_residual, void* d_out,
+               int32_t out_dtype, int64_t ld_out, void* stream) try {
+  if (!ctx) return C4S_ERR_INVALID;
+  if (M < 0 || N < 1 || K < 8 || K % 8) return fail(ctx, C4S_ERR_INVALID, "need M >= 0, N >= 1 and K a multiple of 8");
+  if (dtype != C4S_BF16 && dtype != C4S_FP16) return fail(ctx, C4S_ERR_INVALID, "x and the weight are bf16 or fp16");
+  if (out_dtype != dtype && out_dtype != C4S_FP32) return fail(ctx, C4S_ERR_INVALID, "out is of x's type or fp32");
+  if (act < C4S_ACT_NONE || act > C4S_ACT_RELU) return fail(ctx, C4S_ERR_INVALID, "unknown activation");
+  if (M == 0) return C4S_OK;
+  if (!d_x || !d_weight || !d_out) return fail(ctx, C4S_ERR_INVALID, "null pointer");
+  if (M == 1) {                                    // one row: its stride says nothing
+    ld_x = K;
+    ld_out = ld_residual = 0;
+  }
+  if (N == 1) ld_weight = K;
+  if ((M > 1 && (ld_x < K || ld_out < N || (d_residual && ld_residual < N))) || ld_weight < K)
+    return fail(ctx, C4S_ERR_INVALID, "row stride below the row length");
+  if (d_norm && (K > 8 * 8 * c4s::LNORM_NT || ((uintptr_t)d_norm & 15)))
+    return fail(ctx, C4S_ERR_INVALID, "the LayerNorm needs K <= 8192 and an aligned workspace");
+  if (d_norm && !(eps >= 0.0f)) return fail(ctx, C4S_ERR_INVALID, "eps must not be negative");
+  const uintptr_t os = out_dtype == C4S_FP32 ? 4 : 2;
+  if (((uintptr_t)d_weight & 15) || (ld_weight & 7) || (!d_norm && (((uintptr_t)d_x & 15) || (ld_x & 7))) ||
+      ((uintptr_t)d_x & 1) || ((uintptr_t)d_out & (os - 1)) || ((uintptr_t)d_residual & (os - 1)))
+    return fail(ctx, C4S_ERR_INVALID, "misaligned pointer or stride (TMA needs 16-byte rows)");
+  if ((long long)M > 65535LL * c4s::LN_BM) return fail(ctx, C4S_ERR_CAPACITY, "M above 8388480");
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok) return fail(ctx, C4S_ERR_CUDA, "cannot select the context's device");
+  cudaError_t e;
+  if (d_norm) {
+    e = dtype == C4S_BF16 ? launch_norm<__nv_bfloat16>(d_x, M, K, ld_x, d_gamma, d_beta, eps, d_norm, stream)
+                          : launch_norm<__half>(d_x, M, K, ld_x, d_gamma, d_beta, eps, d_norm, stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "norm launch");
+    d_x = d_norm;
+    ld_x = K;
+  }
+  // tiles of 128 columns where they fill the machine, else of 64, and clusters that share a tile's K
+  const int mt = (M + c4s::LN_BM - 1) / c4s::LN_BM, KB = (K + c4s::LN_BK - 1) / c4s::LN_BK;
+  const int bn = (long long)mt * ((N + 127) / 128) >= ctx->num_sms ? 128 : 64;
+  const long long nt = (N + bn - 1) / bn;
+  int S = 1;
+  while (S < 8 && nt * mt * S * 2 <= ctx->num_sms + ctx->num_sms / 4 && KB >= S * 2 * 4) S *= 2;
+  const int box = std::min(c4s::LN_BM, (M + 7) / 8 * 8);
+  CUtensorMap tx, tw;
+  if (!encode_rows(&tx, dtype, d_x, K, M, ld_x * 2, box) ||
+      !encode_rows(&tw, dtype, d_weight, K, N, ld_weight * 2, bn))
+    return fail(ctx, C4S_ERR_CUDA, "tensor map encoding failed");
+  c4s::LinArgs a;
+  a.bias = d_bias;
+  a.residual = d_residual;
+  a.ldr = ld_residual;
+  a.out = d_out;
+  a.ldo = ld_out;
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.act = act;
+  a.vec_out = ((uintptr_t)d_out & 15) == 0 && (ld_out * os) % 16 == 0;
+  a.vec_res = ((uintptr_t)d_residual & 15) == 0 && (ld_residual * os) % 16 == 0;
+  a.xbytes = (unsigned)box * c4s::LN_BK * 2;
+  a.errflags = ctx->d_err;
+  const TilePick k = dtype == C4S_BF16
+                         ? (out_dtype == C4S_FP32 ? tile_pick<__nv_bfloat16, float>(bn) : tile_pick<__nv_bfloat16, __nv_bfloat16>(bn))
+                         : (out_dtype == C4S_FP32 ? tile_pick<__half, float>(bn) : tile_pick<__half, __half>(bn));
+  e = cudaFuncSetAttribute(k.kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem);
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "linear kernel attribute");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(nt * S), (unsigned)mt);
+  cfg.blockDim = dim3(c4s::LN_THREADS);
+  cfg.dynamicSmemBytes = k.smem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)S;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = S > 1 ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, k.kern, tx, tw, a, S);
+  return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "linear launch");
 } catch (...) {
   return C4S_ERR_INVALID;
 }

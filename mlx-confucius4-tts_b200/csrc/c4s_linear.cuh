@@ -1,0 +1,341 @@
+// c4s_linear.cuh -- the linear layer of the GPT-2 blocks on sm_100a tensor
+// cores, with what surrounds it in the same call:
+//
+//     y = act(LN(x) W^T + b) + r
+//
+// (nn.cpp:11-16 linear, nn.cpp:73-83 layer_norm, the blocks' GELU and residual
+// adds), bf16 or fp16 operands, fp32 accumulation, bias, activation and
+// residual in fp32, one rounding at the store.
+//
+// lin_tile_kernel: one CTA per 128 x BN tile of the output (a TMA producer
+// warp, one MMA-issuing lane, eight epilogue warps; a ring of 64-wide k-blocks
+// in 128-byte-swizzled shared memory, the accumulator in TMEM). Where the
+// tiles are fewer than the SMs, a cluster of S CTAs shares a tile: each takes
+// a part of K, leaves its fp32 partial in its own shared memory, and sums a
+// share of the rows over the cluster in a fixed order.
+#pragma once
+
+#include "c4s_tc.cuh"
+
+namespace c4s {
+
+constexpr int LN_BM = 128, LN_BK = 64;
+constexpr int LN_EPI_WARPS = 8;
+constexpr int LN_THREADS = 64 + 32 * LN_EPI_WARPS;
+constexpr int LN_STAGE_PITCH = 36;                 // floats per row of a warp's 32 x 32 staging block (16-byte rows,
+                                                   // eight rows on different banks)
+
+struct LinArgs {
+  const float* bias;                               // [N] or null
+  const void* residual;                            // [M, ldr] of the output's type, or null
+  long long ldr;
+  void* out;                                       // [M, ldo]
+  long long ldo;
+  int M, N, K;
+  int act;                                         // C4S_ACT_*
+  bool vec_out, vec_res;                           // 16-byte aligned rows
+  unsigned xbytes;                                 // bytes of one TMA box of x
+  unsigned* errflags;
+};
+
+__device__ __forceinline__ float activate(float x, int act) {
+  switch (act) {
+    case C4S_ACT_GELU: {
+      // 0.5 x (1 + tanh u) = x / (1 + e^(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
+      const float u = 0.7978845608028654f * fmaf(0.044715f * x, x * x, x);
+      return x / (1.0f + __expf(-2.0f * u));
+    }
+    case C4S_ACT_GELU_ERF: return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+    case C4S_ACT_SILU: return x / (1.0f + __expf(-x));
+    case C4S_ACT_RELU: return x < 0.0f ? 0.0f : x;   // NaN stays
+    default: return x;
+  }
+}
+
+// NV consecutive outputs of a row from column n: residual, rounding, store.
+template <typename TO, int NV>
+__device__ __forceinline__ void lin_store(const LinArgs& a, long long row, int n, float (&v)[NV]) {
+  static_assert(NV * sizeof(TO) == 16, "one 16-byte store");
+  TO* o = static_cast<TO*>(a.out) + row * a.ldo + n;
+  const bool full = n + NV <= a.N;
+  if (a.residual) {
+    const TO* r = static_cast<const TO*>(a.residual) + row * a.ldr + n;
+    if (full && a.vec_res) {
+      TO x[NV];
+      *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(r);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i] += Cvt<TO>::f(x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (n + i < a.N) v[i] += Cvt<TO>::f(r[i]);
+    }
+  }
+  if (full && a.vec_out) {
+    __align__(16) TO x[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = Cvt<TO>::t(v[i]);
+    *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (n + i < a.N) o[i] = Cvt<TO>::t(v[i]);
+  }
+}
+
+// A warp's 32 x 32 block of finished values (fp32, row pitch LN_STAGE_PITCH)
+// to the output: NV columns a lane, whole 16-byte pieces of rows.
+template <typename TO>
+__device__ __forceinline__ void lin_store_block(const LinArgs& a, const float* st, long long m0, int n0, int lane) {
+  constexpr int NV = 16 / sizeof(TO), LPR = 32 / NV, RPI = 32 / LPR;   // lanes per row, rows per pass
+  const int c = (lane % LPR) * NV;
+#pragma unroll
+  for (int i = 0; i < 32 / RPI; ++i) {
+    const int r = i * RPI + lane / LPR;
+    if (m0 + r < a.M && n0 + c < a.N) {
+      float v[NV];
+#pragma unroll
+      for (int j = 0; j < NV; j += 4)
+        *reinterpret_cast<float4*>(&v[j]) = *reinterpret_cast<const float4*>(st + r * LN_STAGE_PITCH + c + j);
+      lin_store<TO, NV>(a, m0 + r, n0 + c, v);
+    }
+  }
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float4 ld_cluster(unsigned addr, unsigned rank) {
+  unsigned p;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(p) : "memory");
+  return v;
+}
+
+template <int BN>
+struct LinCfg {
+  static constexpr unsigned XB = LN_BM * LN_BK * 2, WB = BN * LN_BK * 2;   // bytes of a stage's tiles
+  static constexpr int STAGES = BN <= 64 ? 8 : 6;
+  static constexpr int PPITCH = BN + 4;                                    // floats per row of a split tile's partial
+  static constexpr size_t SMEM = STAGES * (size_t)(XB + WB) + 1024;
+  static_assert((size_t)LN_BM * PPITCH * 4 <= STAGES * (size_t)(XB + WB), "the partial fits the ring");
+  static_assert((size_t)LN_EPI_WARPS * 32 * LN_STAGE_PITCH * 4 <= STAGES * (size_t)(XB + WB), "and the staging blocks");
+};
+
+// TI: operands; TO: output; grid (ceil(N / BN) S, ceil(M / 128)), clusters of S along x.
+template <typename TI, typename TO, int BN>
+__global__ void __launch_bounds__(LN_THREADS, 1) lin_tile_kernel(const __grid_constant__ CUtensorMap tmX,
+                                                                 const __grid_constant__ CUtensorMap tmW, LinArgs a,
+                                                                 int S) {
+  using Cfg = LinCfg<BN>;
+  constexpr int ST = Cfg::STAGES;
+  constexpr unsigned BF = std::is_same<TI, __nv_bfloat16>::value ? 1u : 0u;
+  constexpr unsigned IDESC = (1u << 4) | (BF << 7) | (BF << 10) | ((unsigned)(BN >> 3) << 17) | ((unsigned)(LN_BM >> 4) << 24);
+  extern __shared__ unsigned char lsm_raw[];
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<unsigned long long>(lsm_raw) + 1023ull) & ~1023ull);
+  __shared__ unsigned long long full[ST], empty[ST], accum;
+  __shared__ unsigned tmem_base;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int s = (int)(blockIdx.x % (unsigned)S);
+  const int n0 = (int)(blockIdx.x / (unsigned)S) * BN, m0 = blockIdx.y * LN_BM;
+  const int KB = (a.K + LN_BK - 1) / LN_BK;
+  const int k0 = (int)((long long)KB * s / S), k1 = (int)((long long)KB * (s + 1) / S);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&accum, 1);
+    abort_flag = 0;
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_base, BN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = tmem_base;
+  grid_dep_wait();                                 // x (the norm's output among it) and the residual
+  grid_dep_launch();
+  auto give_up = [&]() {
+    atomicOr(a.errflags, C4S_DEVERR_TIMEOUT);
+    abort_flag = 1;
+  };
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      for (; it < k1 - k0 && !abort_flag; ++it) {
+        const int i = it % ST;
+        if (!mbar_wait_1s(&empty[i], ((unsigned)(it / ST) & 1u) ^ 1u)) { give_up(); break; }
+        unsigned char* sx = ring + (size_t)i * (Cfg::XB + Cfg::WB);
+        mbar_arrive_expect_tx(&full[i], a.xbytes + Cfg::WB);
+        tma_load_2d(sx, &tmX, (k0 + it) * LN_BK, m0, &full[i]);
+        tma_load_2d(sx + Cfg::XB, &tmW, (k0 + it) * LN_BK, n0, &full[i]);
+      }
+      // after a wait that gave up: the copies in flight land before the CTA goes
+      if (abort_flag)
+        for (int j = max(0, it - ST); j < it; ++j) mbar_wait_1s(&full[j % ST], (unsigned)(j / ST) & 1u);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int it = 0; it < k1 - k0 && !abort_flag; ++it) {
+        const int i = it % ST;
+        if (!mbar_wait_1s(&full[i], (unsigned)(it / ST) & 1u)) { give_up(); break; }
+        tc_fence_after();
+        const unsigned char* sx = ring + (size_t)i * (Cfg::XB + Cfg::WB);
+        const unsigned long long xd = sw128_desc(sx), wd = sw128_desc(sx + Cfg::XB);
+#pragma unroll
+        for (int kk = 0; kk < LN_BK / 16; ++kk)
+          umma_f16(tmem, xd + 2ull * kk, wd + 2ull * kk, IDESC, (it | kk) != 0 ? 1u : 0u);
+        umma_commit(&empty[i]);
+      }
+      umma_commit(&accum);
+    }
+    __syncwarp();
+  } else {
+    const bool ok = mbar_wait_1s(&accum, 0u);
+    if (!ok) give_up();
+    tc_fence_after();
+    __syncwarp();
+    const int q = warp & 3, half = (warp - 2) >> 2;           // TMEM lane quarter; which column chunks
+    const int rows = min(LN_BM, a.M - m0);
+    if (ok && !abort_flag && k1 > k0 && 32 * q < rows) {
+      for (int c = half; c < BN / 32; c += 2) {
+        unsigned r[32];
+        tmem_ld32(tmem + ((unsigned)(32 * q) << 16) + (unsigned)(32 * c), r);
+        tmem_ld_wait();
+        if (S == 1) {
+          // lane = row: bias and activation, through the warp's staging block (in the idle ring) to whole rows
+          float* st = reinterpret_cast<float*>(ring) + (warp - 2) * 32 * LN_STAGE_PITCH;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            float4 v;
+            float* pv = &v.x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int n = n0 + 32 * c + j + e;
+              pv[e] = activate(__uint_as_float(r[j + e]) + (a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f), a.act);
+            }
+            *reinterpret_cast<float4*>(st + lane * LN_STAGE_PITCH + j) = v;
+          }
+          __syncwarp();
+          lin_store_block<TO>(a, st, (long long)m0 + 32 * q, n0 + 32 * c, lane);
+          __syncwarp();
+        } else {
+          float* p = reinterpret_cast<float*>(ring) + (32 * q + lane) * Cfg::PPITCH + 32 * c;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(p + j) = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
+                                                            __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, BN);
+  }
+  if (S > 1) {
+    // every CTA of the cluster passes both barriers, also after a wait that gave up
+    cluster_arrive();
+    cluster_wait();
+    const int rows = min(LN_BM, a.M - m0);
+    const int r0 = rows * s / S, r1 = rows * (s + 1) / S;     // this CTA's share of the rows
+    constexpr int CG = BN / 4;                                // 4 columns a thread
+    if (!abort_flag) {
+      for (int i = threadIdx.x; i < (r1 - r0) * CG; i += LN_THREADS) {
+        const int r = r0 + i / CG, c = (i % CG) * 4;
+        if (n0 + c >= a.N) continue;
+        const unsigned addr = smem_u32(ring) + (unsigned)(r * Cfg::PPITCH + c) * 4u;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int p = 0; p < S; ++p) {
+          const float4 x = ld_cluster(addr, (unsigned)p);
+          v[0] += x.x;
+          v[1] += x.y;
+          v[2] += x.z;
+          v[3] += x.w;
+        }
+        const long long row = (long long)m0 + r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = n0 + c + e;
+          if (n >= a.N) break;
+          float y = activate(v[e] + (a.bias ? __ldg(a.bias + n) : 0.0f), a.act);
+          if (a.residual) y += Cvt<TO>::f(static_cast<const TO*>(a.residual)[row * a.ldr + n]);
+          static_cast<TO*>(a.out)[row * a.ldo + n] = Cvt<TO>::t(y);
+        }
+      }
+    }
+    cluster_arrive();
+    cluster_wait();                                // no CTA leaves while another reads its partial
+  }
+}
+
+// LayerNorm of the rows (nn.cpp:73-83: biased variance, (x - mean) / sqrt(var
+// + eps) gamma + beta) into the GEMM's operand, rounded to its type: one CTA
+// per row, VPT vectors of 8 elements a thread in registers, two passes over
+// them in fp32.
+constexpr int LNORM_NT = 128;
+template <typename T, int VPT>
+__global__ void __launch_bounds__(LNORM_NT) lin_norm_kernel(const T* __restrict__ x, long long ldx, int K, bool vec,
+                                                            const float* __restrict__ gamma,
+                                                            const float* __restrict__ beta, float eps,
+                                                            T* __restrict__ y) {
+  __shared__ float red[2][LNORM_NT / 32];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const T* xr = x + (long long)blockIdx.x * ldx;
+  T* yr = y + (long long)blockIdx.x * K;
+  float f[VPT][8];
+  float s = 0.0f;
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int k = (v * LNORM_NT + threadIdx.x) * 8;
+    T t[8];
+    if (k < K) load8(xr + k, vec, t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[v][i] = k < K ? Cvt<T>::f(t[i]) : 0.0f;
+      s += f[v][i];
+    }
+  }
+  s = warp_reduce(s, [](float a, float b) { return a + b; });
+  if (lane == 0) red[0][warp] = s;
+  __syncthreads();
+  const float mean = ((red[0][0] + red[0][1]) + (red[0][2] + red[0][3])) / (float)K;
+  float q = 0.0f;
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const bool in = (v * LNORM_NT + threadIdx.x) * 8 < K;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[v][i] -= mean;
+      q = in ? fmaf(f[v][i], f[v][i], q) : q;
+    }
+  }
+  q = warp_reduce(q, [](float a, float b) { return a + b; });
+  if (lane == 0) red[1][warp] = q;
+  __syncthreads();
+  const float rs = 1.0f / sqrtf(((red[1][0] + red[1][1]) + (red[1][2] + red[1][3])) / (float)K + eps);
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int k = (v * LNORM_NT + threadIdx.x) * 8;
+    if (k >= K) break;
+    T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      t[i] = Cvt<T>::t(fmaf(f[v][i] * rs, gamma ? __ldg(gamma + k + i) : 1.0f, beta ? __ldg(beta + k + i) : 0.0f));
+    uint4 w;
+    memcpy(&w, t, 16);
+    *reinterpret_cast<uint4*>(yr + k) = w;
+  }
+}
+
+}  // namespace c4s

@@ -127,3 +127,36 @@ def test_null_context_is_refused():
     assert lib.c4s_attention_workspace(None, 1, 1, 64) == -1
     assert lib.c4s_paged_attention(None, s, None, 1, 1, 1, None, 0, 1, 0, 0, None, None, 1.0, None, 0, 0, None, 0,
                                    None) == -1
+
+
+def test_linear_refusals():
+    c4s = load_c4s()
+    chk = c4s.block.check_linear
+    x, w = torch.zeros((3, 64), dtype=torch.bfloat16), torch.zeros((5, 64), dtype=torch.bfloat16)
+    ok = dict(bias=None, act="none", residual=None, gamma=None, beta=None, out=None, out_dtype=None)
+    assert chk(x, w, **ok)[:5] == (3, 64, 5, 0, 0)
+    assert chk(x.half(), w.half(), **{**ok, "out_dtype": torch.float32})[:5] == (3, 64, 5, 1, 2)
+    for change in [dict(out_dtype=torch.float16), dict(residual=torch.zeros((3, 5))),
+                   dict(out=torch.zeros((3, 5), dtype=torch.float16))]:
+        with pytest.raises(TypeError):
+            chk(x, w, **{**ok, **change})
+    for change in [dict(act="tanh"), dict(bias=torch.zeros(4)), dict(bias=torch.zeros(5, dtype=torch.bfloat16)),
+                   dict(gamma=torch.zeros(5)), dict(beta=torch.zeros((64, 1))),
+                   dict(residual=torch.zeros((3, 4), dtype=torch.bfloat16)),
+                   dict(out=torch.zeros((3, 10), dtype=torch.bfloat16)[:, ::2]),
+                   dict(out=torch.zeros((1, 5), dtype=torch.bfloat16).expand(3, 5))]:
+        with pytest.raises(ValueError):
+            chk(x, w, **{**ok, **change})
+    with pytest.raises(TypeError):
+        chk(x.float(), w.float(), **ok)
+    with pytest.raises(TypeError):
+        chk(x, w.half(), **ok)
+    with pytest.raises(ValueError):
+        chk(x[:, :32], w, **ok)
+    with pytest.raises(ValueError):
+        chk(x[0], w, **ok)
+    with pytest.raises(ValueError):
+        chk(x, w.t().contiguous().t(), **ok)
+    lib = c4s.library()
+    assert lib.c4s_linear(None, None, 0, 1, 8, 8, None, None, 1e-5, None, None, 1, 8, None, 0, None, 0, None, 0, 1,
+                          None) == -1

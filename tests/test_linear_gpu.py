@@ -1,0 +1,189 @@
+"""The linear layer with LayerNorm, bias, activation and residual (c4s_linear)
+against fp64 on the same operands.
+
+Tolerance: one rounding of the output (half a step, eps / 2 of its size); the
+fp32 sum of K exact products in blocks of 16 with up to 8 partial sums, each
+add truncated at worst (K / 16 + 24 times 2^-23 of sum |x w|), passed on by
+the activation's slope (below 1.13 for all of them) with 2^-20 of its own;
+with the LayerNorm each operand is rounded once more (eps / 2) and carries
+fp32's error of mean and variance (2^-20).
+"""
+import math
+
+import pytest
+
+from conftest import load_c4s
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
+DEV = "cuda:0"
+F = torch.nn.functional
+ACTS = {"none": lambda y: y, "gelu": lambda y: F.gelu(y, approximate="tanh"), "gelu_erf": F.gelu,
+        "silu": F.silu, "relu": F.relu}
+
+
+@pytest.fixture(scope="module")
+def c4s():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return load_c4s()
+
+
+@pytest.fixture(scope="module")
+def ctx(c4s):
+    return c4s.SamplingContext(max_vocab=64, device=0, max_rows=1)
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def check(ctx, x, w, out, bias=None, act="none", residual=None, layer_norm=False, gamma=None, beta=None, eps=1e-5):
+    xd, wd = x.double(), w.double()
+    K = x.shape[1]
+    extra = 0.0
+    if layer_norm:
+        mean = xd.mean(1, keepdim=True)
+        xd = (xd - mean) / torch.sqrt(((xd - mean) ** 2).mean(1, keepdim=True) + eps)
+        size = xd.abs()
+        if gamma is not None:
+            xd, size = xd * gamma.double(), size * gamma.double().abs()
+        if beta is not None:
+            xd, size = xd + beta.double(), size + beta.double().abs()
+        extra = (xd.abs() * torch.finfo(x.dtype).eps / 2 * 1.001 + size * 2.0 ** -20) @ wd.abs().T
+    y = xd @ wd.T
+    b = 0 if bias is None else bias.double()
+    ref = ACTS[act](y + b)
+    slope = 1.0 if act in ("none", "relu") else 1.13
+    acc = slope * ((xd.abs() @ wd.abs().T) * (K / 16 + 24) * 2.0 ** -23 + extra + (y + b).abs() * 2.0 ** -23)
+    acc = acc + 2.0 ** -20 * ref.abs() + (0 if act in ("none", "relu") else 2.0 ** -21)
+    if residual is not None:
+        ref = ref + residual.double()
+    half = torch.finfo(out.dtype).eps / 2
+    bound = ref.abs() * half * 1.001 + acc * (1 + half) + torch.finfo(out.dtype).smallest_normal
+    err = (out.double() - ref).abs()
+    assert torch.all(err <= bound), float((err / bound).max())
+    assert ctx.status()[0] == 0
+
+
+def operands(M, K, N, dtype, g):
+    x = (torch.randn((M, K), generator=g, device=DEV) * 1.5 + 0.1).to(dtype)
+    w = (torch.randn((N, K), generator=g, device=DEV) / math.sqrt(K)).to(dtype)
+    return x, w
+
+
+SHAPES = [(1, 1280, 3840), (1, 5120, 1280), (2, 8, 1), (3, 64, 65), (5, 200, 129), (8, 1280, 5120), (9, 5120, 640),
+          (16, 1272, 77), (17, 320, 1280), (64, 5120, 1280), (65, 1280, 1000), (128, 2048, 256), (200, 72, 3333),
+          (256, 1280, 5120), (300, 4104, 130), (1000, 640, 2000), (2049, 1280, 1281)]
+
+
+@pytest.mark.parametrize("dtype,odt", [(BF, BF), (FP, FP), (BF, F32), (FP, F32)])
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_plain_and_full(ctx, M, K, N, dtype, odt):
+    g = gen(M + K + N)
+    x, w = operands(M, K, N, dtype, g)
+    check(ctx, x, w, ctx.linear(x, w, out_dtype=odt))
+    bias = torch.randn(N, generator=g, device=DEV) * 0.2
+    res = (torch.randn((M, N), generator=g, device=DEV) * 2).to(odt)
+    gamma, beta = 1 + 0.1 * torch.randn(K, generator=g, device=DEV), 0.1 * torch.randn(K, generator=g, device=DEV)
+    kw = dict(bias=bias, act="gelu", residual=res, layer_norm=True, gamma=gamma, beta=beta)
+    check(ctx, x, w, ctx.linear(x, w, out_dtype=odt, **kw), **kw)
+
+
+@pytest.mark.parametrize("M", [1, 40, 700])
+@pytest.mark.parametrize("act", list(ACTS))
+def test_activations(ctx, act, M):
+    g = gen(7)
+    x, w = operands(M, 512, 264, FP, g)
+    w = w * 3
+    bias = torch.randn(264, generator=g, device=DEV) * 3
+    out = ctx.linear(x, w, bias=bias, act=act, out_dtype=F32)
+    check(ctx, x, w, out, bias=bias, act=act)
+    far = ctx.linear(x * 50, w * 20, act=act, out_dtype=F32)         # far into both tails
+    check(ctx, x * 50, w * 20, far, act=act)
+
+
+@pytest.mark.parametrize("M", [1, 6, 33, 513])
+@pytest.mark.parametrize("gamma,beta", [(False, False), (True, False), (False, True)])
+def test_norm_parts(ctx, M, gamma, beta):
+    g = gen(8)
+    for K in (8, 136, 1280, 8192):
+        x, w = operands(M, K, 96, BF, g)
+        x[0] = 3.0                                                   # a constant row: variance 0
+        ga = torch.randn(K, generator=g, device=DEV) if gamma else None
+        be = torch.randn(K, generator=g, device=DEV) if beta else None
+        norm = torch.empty((M, K), dtype=BF, device=DEV)
+        out = ctx.linear(x, w, layer_norm=True, gamma=ga, beta=be, eps=1e-3, norm_out=norm)
+        check(ctx, x, w, out, layer_norm=True, gamma=ga, beta=be, eps=1e-3)
+
+
+@pytest.mark.parametrize("M", [1, 4, 30, 129, 600])
+def test_strides_and_residual_in_place(ctx, M):
+    g = gen(9)
+    K, N = 192, 150
+    wide = torch.randn((M, K + 24), generator=g, device=DEV).to(BF)
+    x = wide[:, 16:16 + K]
+    w = (torch.randn((N, K + 8), generator=g, device=DEV) / 14).to(BF)[:, :K]
+    buf = torch.randn((M, N + 11), generator=g, device=DEV).to(BF)
+    kept = buf.clone()
+    out = buf[:, 3:3 + N]
+    got = ctx.linear(x, w, residual=out, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    check(ctx, x, w, out, residual=kept[:, 3:3 + N])
+    assert torch.equal(buf[:, :3], kept[:, :3]) and torch.equal(buf[:, 3 + N:], kept[:, 3 + N:])
+    # an x whose rows start anywhere goes through the LayerNorm
+    odd = torch.randn((M, K + 5), generator=g, device=DEV).to(BF)[:, 3:3 + K]
+    check(ctx, odd, w, ctx.linear(odd, w, layer_norm=True), layer_norm=True)
+
+
+@pytest.mark.parametrize("M", [1, 5, 70, 400])
+def test_non_finite_rows_stay_apart(ctx, M):
+    g = gen(10)
+    x, w = operands(M, 256, 200, BF, g)
+    clean = ctx.linear(x, w)
+    x[M - 1, 7] = float("nan")
+    out = ctx.linear(x, w, act="relu")
+    assert torch.isnan(out[M - 1]).all()
+    assert torch.equal(out[:M - 1], clean[:M - 1].clamp(min=0))
+
+
+def test_repeats_streams_and_graphs(ctx):
+    """The same bits every time, on another stream and from a replayed graph; nothing to do for no rows."""
+    g = gen(11)
+    for M in (1, 20, 64, 700):
+        x, w = operands(M, 1280, 1280, BF, g)
+        want = ctx.linear(x, w, act="gelu", layer_norm=True)
+        for _ in range(3):
+            assert torch.equal(want, ctx.linear(x, w, act="gelu", layer_norm=True))
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        out = ctx.linear(x, w, act="gelu", layer_norm=True, stream=st)
+        st.synchronize()
+        assert torch.equal(out, want)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            got = ctx.linear(x, w, act="gelu", layer_norm=True)
+        got.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    assert ctx.linear(x[:0], w).shape == (0, 1280)
+
+
+def test_c_refusals(ctx, c4s):
+    x = torch.zeros((4, 64), dtype=BF, device=DEV)
+    with pytest.raises(c4s.C4SError):
+        ctx.linear(x[:, :60], x[:, :60])                             # K not a multiple of 8
+    with pytest.raises(c4s.C4SError):
+        ctx.linear(torch.zeros((4, 68), dtype=BF, device=DEV)[:, 4:], x)      # rows not on 16 bytes
+    with pytest.raises(c4s.C4SError):
+        ctx.linear(x, x, layer_norm=True, eps=-1.0)
+    big = torch.zeros((1, 8200), dtype=BF, device=DEV)
+    with pytest.raises(c4s.C4SError):
+        ctx.linear(big, big, layer_norm=True)
+    with pytest.raises(ValueError):
+        ctx.linear(x.cpu(), x)
+    assert ctx.status()[0] == 0
