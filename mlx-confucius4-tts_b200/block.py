@@ -4,16 +4,16 @@ layer with its epilogue. BlockOps holds the calls (SamplingContext has them),
 KVCache describes a cache's tensors. The C ABI in include/c4s_sampling.h
 defines each operator.
 
-Arguments are checked here (ValueError, TypeError) before the C call, whose own
-refusals raise C4SError. Calls are ordered on the current torch stream of the
-context's device, or on `stream`; with `stream` the outputs that a call
-allocates belong to that stream.
+Arguments are checked by the compiled binding (ValueError, TypeError) before
+the C call, whose own refusals raise C4SError. Calls are ordered on the current
+torch stream of the context's device, or on `stream`; with `stream` the outputs
+that a call allocates belong to that stream.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
-import math
+import importlib.util
+import os
 
 BF16, FP16, FP32 = 0, 1, 2
 HEAD_DIMS = (64, 96, 128)
@@ -48,28 +48,25 @@ def _torch():
     return torch
 
 
-def _type(t, what: str, fp32: bool = False) -> int:
-    """c4s_dtype of a tensor; int16 / uint16 tensors hold bf16 bit patterns."""
-    torch = _torch()
-    kinds = {torch.bfloat16: BF16, torch.float16: FP16, torch.int16: BF16, torch.uint16: BF16}
-    if fp32:
-        kinds[torch.float32] = FP32
-    if t.dtype not in kinds:
-        raise TypeError(f"{what}: {t.dtype} is not supported")
-    return kinds[t.dtype]
+_bind = None
 
 
-def _ints(t, what: str, dtype, shape):
-    if t.dtype != dtype:
-        raise TypeError(f"{what} must be {dtype}")
-    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous, of shape {tuple(shape)}")
-
-
-def _on(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the context on {device}")
+def binding():
+    """The compiled binding (csrc/c4s_bind.cpp, built by __graft_entry__.build())."""
+    global _bind
+    if _bind is None:
+        _torch()
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_c4s.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"c4s binding not built: {path} is missing "
+                               "(run `python -c 'import __graft_entry__ as g; g.build()'`)")
+        spec = importlib.util.spec_from_file_location("_c4s", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        from .sampling import C4SError
+        mod.set_error(C4SError)
+        _bind = mod
+    return _bind
 
 
 class KVCache:
@@ -98,7 +95,9 @@ class KVCache:
         if bits == 16:
             if k_sb is not None or v_sb is not None:
                 raise ValueError("a 16-bit cache has no scales")
-            s.dtype = _type(k, "cache")
+            if k.dtype not in (torch.bfloat16, torch.float16):
+                raise TypeError("16-bit cache rows are bf16 or fp16")
+            s.dtype = FP16 if k.dtype == torch.float16 else BF16
             s.head_dim, s.group = k.shape[3], 0
         else:
             if k.dtype != torch.uint8:
@@ -120,6 +119,10 @@ class KVCache:
             s.sb_page_stride, s.sb_head_stride, s.sb_token_stride = (4 * x for x in k_sb.stride()[:3])
         if s.head_dim not in HEAD_DIMS:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}")
+        for t in (v, k_sb, v_sb):
+            if t is not None and t.device != k.device:
+                raise ValueError("a cache's tensors are on one device")
+        self.address, self.device_index = C.addressof(s), k.get_device()
         s.k, s.v = k.data_ptr(), v.data_ptr()
         s.page_stride, s.head_stride, s.token_stride = (k.element_size() * x for x in k.stride()[:3])
 
@@ -154,159 +157,97 @@ class KVCache:
     def page_size(self):
         return self.struct.page_size
 
-    def _check_table(self, table):
-        torch = _torch()
-        if table.dtype != torch.int32:
-            raise TypeError("page_table must be int32")
-        if table.dim() != 2 or table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1) or \
-                (table.shape[0] > 1 and table.stride(0) < table.shape[1]):
-            raise ValueError("page_table must be [sequences, pages] with contiguous rows")
-
-
-def _rows(t, what: str, heads: int, dim: int):
-    """Checks a [n, heads, dim] tensor with contiguous rows."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
-        raise ValueError(f"{what} must be [n, {heads}, {dim}]")
-    if t.stride(2) != 1 or t.stride(0) < 0 or t.stride(1) < 0:
-        raise ValueError(f"{what}: rows must be contiguous")
-
 
 def check_kv(cache: KVCache, page_table, k, v, pos, tok_off, write: bool):
-    """Refuses what c4s_kv_write / c4s_kv_read cannot take; returns (B, T, c4s_dtype)."""
-    torch = _torch()
-    cache._check_table(page_table)
-    B, T = page_table.shape[0], k.shape[0]
-    _rows(k, "k", cache.kv_heads, cache.head_dim)
-    if k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
-        raise ValueError("k and v must be alike")
-    kind = _type(k, "k", fp32=not write)
-    if write and cache.bits == 16 and kind != cache.struct.dtype:
-        raise TypeError("k and v must be of the cache's type")
-    if not write and (k.stride(1) < cache.head_dim or (T > 1 and k.stride(0) < cache.head_dim)) and cache.kv_heads > 1:
-        raise ValueError("the rows of k and v must not overlap")
-    _ints(pos, "pos", torch.int32, (B,))
-    if tok_off is None:
-        if T != B:
-            raise ValueError("without tok_off there is one token per sequence")
-    else:
-        _ints(tok_off, "tok_off", torch.int64, (B + 1,))
-    return B, T, kind
+    """Refuses what kv_write (write) and kv_read cannot take; (B, T, c4s_dtype)."""
+    return binding().check_kv(cache.address, page_table, k, v, pos, tok_off, write)
 
 
 def check_attention(q, cache: KVCache, page_table, lens, start, out):
-    """Refuses what c4s_paged_attention cannot take; returns (B, q_heads, c4s_dtype)."""
-    torch = _torch()
-    cache._check_table(page_table)
-    B = page_table.shape[0]
-    if q.dim() != 3 or q.shape[0] != B or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
-        raise ValueError("q must be [sequences, q_heads, head_dim], q_heads a multiple of the cache's heads")
-    _rows(q, "q", q.shape[1], cache.head_dim)
-    kind = _type(q, "q")
-    if cache.bits == 16 and kind != cache.struct.dtype:
-        raise TypeError("q must be of the cache's type")
-    _ints(lens, "lens", torch.int32, (B,))
-    if start is not None:
-        _ints(start, "start", torch.int32, (B,))
-    if out is not None:
-        _rows(out, "out", q.shape[1], cache.head_dim)
-        if out.shape != q.shape or out.dtype != q.dtype:
-            raise ValueError("out must be like q")
-        if (B > 1 and out.stride(0) < cache.head_dim) or (q.shape[1] > 1 and out.stride(1) < cache.head_dim):
-            raise ValueError("the rows of out must not overlap")
-    return B, q.shape[1], kind
-
-
-def _matrix(t, what: str, shape):
-    if t.dim() != 2 or tuple(t.shape) != tuple(shape) or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what} must be {tuple(shape)} with contiguous rows")
+    """Refuses what paged_attention cannot take; (B, q_heads, c4s_dtype)."""
+    return binding().check_attention(cache.address, q, page_table, lens, start, out)
 
 
 def check_linear(x, weight, bias, act, residual, gamma, beta, out, out_dtype):
-    """Refuses what c4s_linear cannot take; returns (M, K, N, c4s_dtype of x, of out, torch type of out)."""
-    torch = _torch()
-    if x.dim() != 2 or weight.dim() != 2:
-        raise ValueError("x must be [M, K] and weight [N, K]")
-    M, K = x.shape
-    N = weight.shape[0]
-    _matrix(x, "x", (M, K))
-    _matrix(weight, "weight", (N, K))
-    kind = _type(x, "x")
-    if _type(weight, "weight") != kind:
-        raise TypeError("x and weight must be of one type")
+    """Refuses what linear cannot take; (M, K, N, c4s_dtype of x, of out)."""
+    _activation(act)
+    return binding().check_linear(x, weight, bias, residual, gamma, beta, out, _out_code(x, out_dtype))
+
+
+def _activation(act: str) -> int:
     if act not in ACTIVATIONS:
         raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}")
+    return ACTIVATIONS[act]
+
+
+def _out_code(x, out_dtype) -> int:
     if out_dtype is None:
-        out_dtype = x.dtype if out is None else out.dtype
-    okind = FP32 if out_dtype == torch.float32 else kind
-    if out_dtype != torch.float32 and out_dtype != x.dtype:
+        return 0
+    if out_dtype == x.dtype:
+        return 1
+    if str(out_dtype) != "torch.float32":
         raise TypeError("out is of x's type or fp32")
-    for name, t, n in (("bias", bias, N), ("gamma", gamma, K), ("beta", beta, K)):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (n,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous fp32 [{n}]")
-    for name, t in (("residual", residual), ("out", out)):
-        if t is not None:
-            if t.dtype != out_dtype:
-                raise TypeError(f"{name} must be {out_dtype}")
-            _matrix(t, name, (M, N))
-    if M > 1 and out is not None and out.stride(0) < N:
-        raise ValueError("the rows of out must not overlap")
-    return M, K, N, kind, okind, out_dtype
+    return 2
 
 
 class BlockOps:
     """The block's operators of a context (SamplingContext)."""
 
-    def _allocating(self, stream):
-        """New tensors belong to the stream that the call runs on."""
-        return contextlib.nullcontext() if stream is None else _torch().cuda.stream(stream)
+    def _on_stream(self, stream, call, *args, **kw):
+        """`call` with `stream` as the current one, so that its outputs belong to it."""
+        if stream.device.index != (self.device.index or 0):
+            raise ValueError(f"the stream is on {stream.device}, the context on {self.device}")
+        with _torch().cuda.stream(stream):
+            return call(*args, **kw)
+
+    def _handle(self):
+        if not self._h:
+            raise RuntimeError("the context is closed")
+        return self._h.value
 
     def kv_write(self, cache: KVCache, page_table, k, v, pos, tok_off=None, stream=None):
         """Writes new tokens' k, v [T, kv_heads, head_dim] into the cache
         (c4s_kv_write). page_table int32 [B, pages]; pos int32 [B], the position
         of each sequence's first new token (< 0: skip it); tok_off int64 [B+1],
         the sequences' tokens, or None for one token per sequence."""
-        B, T, kind = check_kv(cache, page_table, k, v, pos, tok_off, True)
-        _on(self.device, k=k, v=v, page_table=page_table, pos=pos, tok_off=tok_off, cache=cache.k)
-        rc = self.lib.c4s_kv_write(
-            self._h, C.byref(cache.struct), page_table.data_ptr(), page_table.stride(0), page_table.shape[1], B,
-            k.data_ptr(), v.data_ptr(), kind, k.stride(0), k.stride(1), T,
-            None if tok_off is None else tok_off.data_ptr(), pos.data_ptr(), self._stream(stream))
-        self._check(rc, "c4s_kv_write")
+        if stream is not None:
+            return self._on_stream(stream, self.kv_write, cache, page_table, k, v, pos, tok_off)
+        binding().kv(self._handle(), self.device.index or 0, cache.address, cache.device_index, page_table, k, v, pos,
+                     tok_off, True)
 
     def kv_read(self, cache: KVCache, page_table, pos, tok_off=None, total: int | None = None, dtype=None, k_out=None,
                 v_out=None, stream=None):
         """Reads positions back (c4s_kv_read): (k, v) [total, kv_heads,
         head_dim] of `dtype` (the cache's type, or bf16 for codes), total =
-        tok_off[B] (the sequences, without tok_off)."""
-        torch = _torch()
+        tok_off[B] (the sequences, without tok_off). Rows of skipped sequences
+        and behind tok_off[B] are left as they were."""
+        if stream is not None:
+            return self._on_stream(stream, self.kv_read, cache, page_table, pos, tok_off, total, dtype, k_out, v_out)
         if (k_out is None) != (v_out is None):
             raise ValueError("k_out and v_out go together")
         if k_out is None:
+            torch = _torch()
             if total is None:
                 if tok_off is not None:
                     raise ValueError("total is needed with tok_off")
                 total = page_table.shape[0]
             if dtype is None:
-                dtype = torch.float16 if cache.bits == 16 and cache.struct.dtype == FP16 else torch.bfloat16
-            with self._allocating(stream):
-                k_out, v_out = (torch.empty((total, cache.kv_heads, cache.head_dim), dtype=dtype, device=self.device)
-                                for _ in "kv")
-        B, T, kind = check_kv(cache, page_table, k_out, v_out, pos, tok_off, False)
-        _on(self.device, k_out=k_out, v_out=v_out, page_table=page_table, pos=pos, tok_off=tok_off, cache=cache.k)
-        rc = self.lib.c4s_kv_read(
-            self._h, C.byref(cache.struct), page_table.data_ptr(), page_table.stride(0), page_table.shape[1], B,
-            k_out.data_ptr(), v_out.data_ptr(), kind, k_out.stride(0), k_out.stride(1), T,
-            None if tok_off is None else tok_off.data_ptr(), pos.data_ptr(), self._stream(stream))
-        self._check(rc, "c4s_kv_read")
+                dtype = torch.bfloat16 if cache.bits != 16 else cache.k.dtype
+            s = cache.struct
+            # one allocation: keys, then values
+            k_out, v_out = torch.empty((2, total, s.kv_heads, s.head_dim), dtype=dtype, device=self.device).unbind(0)
+        binding().kv(self._handle(), self.device.index or 0, cache.address, cache.device_index, page_table, k_out, v_out,
+                     pos, tok_off, False)
         return k_out, v_out
 
     def attention_workspace(self, batch: int, q_heads: int, head_dim: int, stream=None):
         """A zeroed workspace for paged_attention. Keep one per stream (or captured graph)."""
+        if stream is not None:
+            return self._on_stream(stream, self.attention_workspace, batch, q_heads, head_dim)
         n = self.lib.c4s_attention_workspace(self._h, batch, q_heads, head_dim)
         if n < 0:
             self._check(int(n), "c4s_attention_workspace")
-        with self._allocating(stream):
-            return _torch().zeros(n, dtype=_torch().uint8, device=self.device)
+        return _torch().zeros(n, dtype=_torch().uint8, device=self.device)
 
     def paged_attention(self, q, cache: KVCache, page_table, lens, start=None, scale: float | None = None, out=None,
                         work=None, stream=None):
@@ -314,23 +255,10 @@ class BlockOps:
         [start, lens) (c4s_paged_attention): q [B, q_heads, head_dim] -> out,
         like q. lens, start int32 [B]; scale 1 / sqrt(head_dim) by default;
         work: attention_workspace() (None: one for this call)."""
-        torch = _torch()
-        B, heads, kind = check_attention(q, cache, page_table, lens, start, out)
-        _on(self.device, q=q, page_table=page_table, lens=lens, start=start, out=out, work=work, cache=cache.k)
-        if out is None:
-            with self._allocating(stream):
-                out = torch.empty((B, heads, cache.head_dim), dtype=q.dtype, device=self.device)
-        if work is None:
-            work = self.attention_workspace(B, heads, cache.head_dim, stream)
-        if scale is None:
-            scale = 1.0 / math.sqrt(cache.head_dim)
-        rc = self.lib.c4s_paged_attention(
-            self._h, C.byref(cache.struct), page_table.data_ptr(), page_table.stride(0), page_table.shape[1], B,
-            q.data_ptr(), kind, heads, q.stride(0), q.stride(1), lens.data_ptr(),
-            None if start is None else start.data_ptr(), scale, out.data_ptr(), out.stride(0), out.stride(1),
-            work.data_ptr(), work.numel() * work.element_size(), self._stream(stream))
-        self._check(rc, "c4s_paged_attention")
-        return out
+        if stream is not None:
+            return self._on_stream(stream, self.paged_attention, q, cache, page_table, lens, start, scale, out, work)
+        return binding().paged_attention(self._handle(), self.device.index or 0, cache.address, cache.device_index, q,
+                                         page_table, lens, start, scale, out, work)
 
     def linear(self, x, weight, bias=None, act: str = "none", residual=None, layer_norm: bool = False, gamma=None,
                beta=None, eps: float = 1e-5, norm_out=None, out=None, out_dtype=None, stream=None):
@@ -339,24 +267,8 @@ class BlockOps:
         gamma, beta fp32; act one of ACTIVATIONS; residual of out's type (it may
         be out); layer_norm=False skips the LayerNorm; norm_out: [M, K] workspace
         of the normalised rows."""
-        torch = _torch()
-        M, K, N, kind, okind, out_dtype = check_linear(x, weight, bias, act, residual, gamma, beta, out, out_dtype)
-        _on(self.device, x=x, weight=weight, bias=bias, residual=residual, gamma=gamma, beta=beta, out=out,
-            norm_out=norm_out)
-        if norm_out is not None:
-            _matrix(norm_out, "norm_out", (M, K))
-            if norm_out.dtype != x.dtype or not norm_out.is_contiguous():
-                raise ValueError("norm_out must be contiguous, of x's type")
-        with self._allocating(stream):
-            if out is None:
-                out = torch.empty((M, N), dtype=out_dtype, device=self.device)
-            if layer_norm and norm_out is None:
-                norm_out = torch.empty((M, K), dtype=x.dtype, device=self.device)
-        rc = self.lib.c4s_linear(
-            self._h, x.data_ptr(), kind, M, K, x.stride(0), None if gamma is None else gamma.data_ptr(),
-            None if beta is None else beta.data_ptr(), eps, norm_out.data_ptr() if layer_norm else None,
-            weight.data_ptr(), N, weight.stride(0), None if bias is None else bias.data_ptr(), ACTIVATIONS[act],
-            None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0),
-            out.data_ptr(), okind, out.stride(0), self._stream(stream))
-        self._check(rc, "c4s_linear")
-        return out
+        if stream is not None:
+            return self._on_stream(stream, self.linear, x, weight, bias, act, residual, layer_norm, gamma, beta, eps,
+                                   norm_out, out, out_dtype)
+        return binding().linear(self._handle(), self.device.index or 0, x, weight, bias, _activation(act), residual,
+                                layer_norm, gamma, beta, eps, norm_out, out, _out_code(x, out_dtype))

@@ -1,0 +1,434 @@
+// c4s_bind.cpp -- Python binding of the decoder block's operators: checks torch
+// tensors and calls the C ABI. A decode step makes several such calls per
+// layer, each a few microseconds on the GPU; checking and passing their twenty
+// arguments through ctypes costs 10 to 17 us of host time a call, here 1 to 2.
+//
+// Plain CPython entry points (METH_FASTCALL, positional arguments; block.py
+// holds the keyword interface). What a call cannot take raises ValueError or
+// TypeError before the device is looked at; a C status raises C4SError.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+#include <limits>
+#include <stdexcept>
+#include <string>
+
+#include "../../include/c4s_sampling.h"
+
+namespace {
+
+using at::Tensor;
+
+PyObject* g_error = nullptr;                       // C4SError
+
+struct Refuse : std::runtime_error {
+  PyObject* type;
+  Refuse(PyObject* t, const std::string& m) : std::runtime_error(m), type(t) {}
+};
+[[noreturn]] void value_error(const std::string& m) { throw Refuse(PyExc_ValueError, m); }
+[[noreturn]] void type_error(const std::string& m) { throw Refuse(PyExc_TypeError, m); }
+
+// A call's arguments, taken in order.
+struct Args {
+  PyObject* const* a;
+  Py_ssize_t n, i = 0;
+  PyObject* next() {
+    if (i >= n) type_error("too few arguments");
+    return a[i++];
+  }
+  const Tensor& tensor(const char* what) {
+    PyObject* o = next();
+    if (!THPVariable_Check(o)) type_error(std::string(what) + " must be a tensor");
+    return THPVariable_Unpack(o);
+  }
+  const Tensor* maybe(const char* what) {
+    PyObject* o = next();
+    if (o == Py_None) return nullptr;
+    if (!THPVariable_Check(o)) type_error(std::string(what) + " must be a tensor or None");
+    return &THPVariable_Unpack(o);
+  }
+  long long integer(const char* what) {
+    const long long v = PyLong_AsLongLong(next());
+    if (v == -1 && PyErr_Occurred()) {
+      PyErr_Clear();
+      type_error(std::string(what) + " must be an integer");
+    }
+    return v;
+  }
+  void* pointer(const char* what) { return reinterpret_cast<void*>(static_cast<intptr_t>(integer(what))); }
+  double real(const char* what) {
+    const double v = PyFloat_AsDouble(next());
+    if (v == -1.0 && PyErr_Occurred()) {
+      PyErr_Clear();
+      type_error(std::string(what) + " must be a number");
+    }
+    return v;
+  }
+};
+
+int kind_of(const Tensor& t, const char* what, bool fp32 = false) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16:
+    case at::kShort:
+    case at::kUInt16: return C4S_BF16;             // bf16, or its bit patterns
+    case at::kHalf: return C4S_FP16;
+    case at::kFloat:
+      if (fp32) return C4S_FP32;
+      [[fallthrough]];
+    default: type_error(std::string(what) + ": this type is not supported");
+  }
+}
+
+int int32_of(int64_t v, const char* what) {
+  if (v < 0 || v > std::numeric_limits<int32_t>::max()) value_error(std::string(what) + " is out of range");
+  return (int)v;
+}
+
+void on(int dev, const Tensor* t, const char* what) {
+  if (t && (!t->is_cuda() || t->get_device() != dev))
+    value_error(std::string(what) + " is not on the context's device");
+}
+
+void ints(const Tensor& t, const char* what, at::ScalarType type, int64_t n) {
+  if (t.scalar_type() != type) type_error(std::string(what) + (type == at::kInt ? " must be int32" : " must be int64"));
+  if (t.dim() != 1 || t.size(0) != n || !t.is_contiguous())
+    value_error(std::string(what) + " must be contiguous, of shape [" + std::to_string(n) + "]");
+}
+
+void table_ok(const Tensor& t) {
+  if (t.scalar_type() != at::kInt) type_error("page_table must be int32");
+  if (t.dim() != 2 || t.size(1) < 1 || (t.size(1) > 1 && t.stride(1) != 1) ||
+      (t.size(0) > 1 && t.stride(0) < t.size(1)))
+    value_error("page_table must be [sequences, pages] with contiguous rows");
+}
+
+// [n, heads, dim] with contiguous rows
+void rows_ok(const Tensor& t, const char* what, int64_t heads, int64_t dim) {
+  if (t.dim() != 3 || t.size(1) != heads || t.size(2) != dim)
+    value_error(std::string(what) + " must be [n, " + std::to_string(heads) + ", " + std::to_string(dim) + "]");
+  if (t.stride(2) != 1 || t.stride(0) < 0 || t.stride(1) < 0) value_error(std::string(what) + ": rows must be contiguous");
+}
+
+// ... that a kernel writes: no two rows in one place
+void apart(const Tensor& t, const char* what) {
+  const int64_t n = t.size(0), h = t.size(1), d = t.size(2), sn = t.stride(0), sh = t.stride(1);
+  const bool ok = (n <= 1 || h <= 1) ? (n <= 1 || sn >= d) && (h <= 1 || sh >= d)
+                                     : (sh >= d && sn >= (h - 1) * sh + d) || (sn >= d && sh >= (n - 1) * sn + d);
+  if (!ok) value_error(std::string("the rows of ") + what + " must not overlap");
+}
+
+[[noreturn]] void c_error(c4s_ctx* ctx, int rc, const char* what) {
+  PyObject* e = PyObject_CallFunction(g_error ? g_error : PyExc_RuntimeError, "is", rc,
+                                      (std::string(what) + ": " + c4s_last_error(ctx)).c_str());
+  if (e) {
+    PyErr_SetObject((PyObject*)Py_TYPE(e), e);
+    Py_DECREF(e);
+  }
+  throw Refuse(nullptr, "");
+}
+
+// Body of an entry point: C++ exceptions become Python ones.
+template <typename F> PyObject* guarded(F&& f) {
+  try {
+    return f();
+  } catch (const Refuse& r) {
+    if (r.type) PyErr_SetString(r.type, r.what());
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
+}
+
+// The current torch stream of the context's device.
+void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
+
+struct KvCall {
+  int B, kind;
+  int64_t T;
+};
+KvCall kv_ok(const c4s_kv_cache& c, const Tensor& table, const Tensor& k, const Tensor& v, const Tensor& pos,
+             const Tensor* off, bool write) {
+  table_ok(table);
+  rows_ok(k, "k", c.kv_heads, c.head_dim);
+  if (k.sizes() != v.sizes() || k.strides() != v.strides() || k.scalar_type() != v.scalar_type())
+    value_error("k and v must be alike");
+  KvCall r{int32_of(table.size(0), "the number of sequences"), kind_of(k, "k", !write), k.size(0)};
+  if (write && c.bits == 16 && r.kind != c.dtype) type_error("k and v must be of the cache's type");
+  if (!write) apart(k, "k and v");
+  ints(pos, "pos", at::kInt, r.B);
+  if (off) ints(*off, "tok_off", at::kLong, (int64_t)r.B + 1);
+  else if (r.T != r.B) value_error("without tok_off there is one token per sequence");
+  return r;
+}
+
+// (ctx, device, cache, cache's device, page_table, k, v, pos, tok_off, write)
+PyObject* kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args a{args, n};
+    c4s_ctx* ctx = static_cast<c4s_ctx*>(a.pointer("context"));
+    const int dev = (int)a.integer("device");
+    const c4s_kv_cache* c = static_cast<const c4s_kv_cache*>(a.pointer("cache"));
+    const long long cdev = a.integer("cache device");
+    const Tensor& table = a.tensor("page_table");
+    const Tensor &k = a.tensor("k"), &v = a.tensor("v"), &pos = a.tensor("pos");
+    const Tensor* off = a.maybe("tok_off");
+    const bool write = a.integer("write") != 0;
+    const KvCall r = kv_ok(*c, table, k, v, pos, off, write);
+    if (cdev != dev) value_error("the cache is not on the context's device");
+    on(dev, &table, "page_table");
+    on(dev, &k, "k");
+    on(dev, &v, "v");
+    on(dev, &pos, "pos");
+    on(dev, off, "tok_off");
+    const int64_t* po = off ? off->const_data_ptr<int64_t>() : nullptr;
+    const int32_t* pp = pos.const_data_ptr<int32_t>();
+    const int32_t* pt = table.const_data_ptr<int32_t>();
+    const int rc = write ? c4s_kv_write(ctx, c, pt, table.stride(0), int32_of(table.size(1), "the page table's width"),
+                                        r.B, k.const_data_ptr(), v.const_data_ptr(), r.kind, k.stride(0), k.stride(1),
+                                        r.T, po, pp, stream_of(dev))
+                         : c4s_kv_read(ctx, c, pt, table.stride(0), int32_of(table.size(1), "the page table's width"),
+                                       r.B, k.data_ptr(), v.data_ptr(), r.kind, k.stride(0), k.stride(1), r.T, po, pp,
+                                       stream_of(dev));
+    if (rc) c_error(ctx, rc, write ? "c4s_kv_write" : "c4s_kv_read");
+    Py_RETURN_NONE;
+  });
+}
+
+// (cache, page_table, k, v, pos, tok_off, write): the checks alone -> (B, T, type)
+PyObject* check_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args a{args, n};
+    const c4s_kv_cache* c = static_cast<const c4s_kv_cache*>(a.pointer("cache"));
+    const Tensor& table = a.tensor("page_table");
+    const Tensor &k = a.tensor("k"), &v = a.tensor("v"), &pos = a.tensor("pos");
+    const Tensor* off = a.maybe("tok_off");
+    const KvCall r = kv_ok(*c, table, k, v, pos, off, a.integer("write") != 0);
+    return Py_BuildValue("iLi", r.B, (long long)r.T, r.kind);
+  });
+}
+
+struct AttnCall {
+  int B, heads, kind;
+};
+AttnCall attention_ok(const c4s_kv_cache& c, const Tensor& q, const Tensor& table, const Tensor& lens,
+                      const Tensor* start, const Tensor* out) {
+  table_ok(table);
+  if (q.dim() != 3 || q.size(0) != table.size(0) || q.size(1) < 1 || q.size(1) % c.kv_heads)
+    value_error("q must be [sequences, q_heads, head_dim], q_heads a multiple of the cache's heads");
+  rows_ok(q, "q", q.size(1), c.head_dim);
+  AttnCall r{int32_of(q.size(0), "the number of sequences"), int32_of(q.size(1), "q_heads"), kind_of(q, "q")};
+  if (c.bits == 16 && r.kind != c.dtype) type_error("q must be of the cache's type");
+  ints(lens, "lens", at::kInt, r.B);
+  if (start) ints(*start, "start", at::kInt, r.B);
+  if (out) {
+    if (out->sizes() != q.sizes() || out->scalar_type() != q.scalar_type()) value_error("out must be like q");
+    rows_ok(*out, "out", r.heads, c.head_dim);
+    apart(*out, "out");
+  }
+  return r;
+}
+
+// (ctx, device, cache, cache's device, q, page_table, lens, start, scale, out, work) -> out
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args a{args, n};
+    c4s_ctx* ctx = static_cast<c4s_ctx*>(a.pointer("context"));
+    const int dev = (int)a.integer("device");
+    const c4s_kv_cache* c = static_cast<const c4s_kv_cache*>(a.pointer("cache"));
+    const long long cdev = a.integer("cache device");
+    const Tensor &q = a.tensor("q"), &table = a.tensor("page_table"), &lens = a.tensor("lens");
+    const Tensor* start = a.maybe("start");
+    PyObject* sc = a.next();
+    double scale = 1.0 / std::sqrt((double)c->head_dim);
+    if (sc != Py_None) {
+      --a.i;
+      scale = a.real("scale");
+    }
+    const Tensor* out = a.maybe("out");
+    const Tensor* work = a.maybe("work");
+    const AttnCall r = attention_ok(*c, q, table, lens, start, out);
+    if (work && !work->is_contiguous()) value_error("work must be contiguous");
+    if (cdev != dev) value_error("the cache is not on the context's device");
+    on(dev, &q, "q");
+    on(dev, &table, "page_table");
+    on(dev, &lens, "lens");
+    on(dev, start, "start");
+    on(dev, out, "out");
+    on(dev, work, "work");
+    Tensor made, scratch;
+    if (!out) {
+      made = at::empty(q.sizes(), q.options());
+      out = &made;
+    }
+    if (!work) {
+      const int64_t bytes = c4s_attention_workspace(ctx, r.B, r.heads, c->head_dim);
+      if (bytes < 0) c_error(ctx, (int)bytes, "c4s_attention_workspace");
+      scratch = at::zeros({bytes}, q.options().dtype(at::kByte));
+      work = &scratch;
+    }
+    const int rc = c4s_paged_attention(
+        ctx, c, table.const_data_ptr<int32_t>(), table.stride(0), int32_of(table.size(1), "the page table's width"),
+        r.B, q.const_data_ptr(), r.kind, r.heads, q.stride(0), q.stride(1), lens.const_data_ptr<int32_t>(),
+        start ? start->const_data_ptr<int32_t>() : nullptr, (float)scale, out->data_ptr(), out->stride(0),
+        out->stride(1), work->data_ptr(), (int64_t)work->nbytes(), stream_of(dev));
+    if (rc) c_error(ctx, rc, "c4s_paged_attention");
+    return THPVariable_Wrap(*out);
+  });
+}
+
+// (cache, q, page_table, lens, start, out): the checks alone -> (B, q_heads, type)
+PyObject* check_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args a{args, n};
+    const c4s_kv_cache* c = static_cast<const c4s_kv_cache*>(a.pointer("cache"));
+    const Tensor &q = a.tensor("q"), &table = a.tensor("page_table"), &lens = a.tensor("lens");
+    const Tensor* start = a.maybe("start");
+    const AttnCall r = attention_ok(*c, q, table, lens, start, a.maybe("out"));
+    return Py_BuildValue("iii", r.B, r.heads, r.kind);
+  });
+}
+
+void matrix_ok(const Tensor& t, const char* what, int64_t m, int64_t n) {
+  if (t.dim() != 2 || t.size(0) != m || t.size(1) != n || (n > 1 && t.stride(1) != 1))
+    value_error(std::string(what) + " must be [" + std::to_string(m) + ", " + std::to_string(n) + "] with contiguous rows");
+}
+void vector_ok(const Tensor* t, const char* what, int64_t n) {
+  if (t && (t->scalar_type() != at::kFloat || t->dim() != 1 || t->size(0) != n || !t->is_contiguous()))
+    value_error(std::string(what) + " must be contiguous fp32 [" + std::to_string(n) + "]");
+}
+
+struct LinCall {
+  int M, K, N, kind, okind;
+  at::ScalarType otype;
+};
+// otype Undefined: out's type, or x's
+LinCall linear_ok(const Tensor& x, const Tensor& w, const Tensor* bias, const Tensor* residual, const Tensor* gamma,
+                  const Tensor* beta, const Tensor* out, at::ScalarType otype) {
+  if (x.dim() != 2 || w.dim() != 2) value_error("x must be [M, K] and weight [N, K]");
+  LinCall r;
+  r.M = int32_of(x.size(0), "M");
+  r.K = int32_of(x.size(1), "K");
+  r.N = int32_of(w.size(0), "N");
+  matrix_ok(x, "x", r.M, r.K);
+  matrix_ok(w, "weight", r.N, r.K);
+  r.kind = kind_of(x, "x");
+  if (kind_of(w, "weight") != r.kind) type_error("x and weight must be of one type");
+  r.otype = otype != at::ScalarType::Undefined ? otype : out ? out->scalar_type() : x.scalar_type();
+  if (r.otype != at::kFloat && r.otype != x.scalar_type()) type_error("out is of x's type or fp32");
+  r.okind = r.otype == at::kFloat ? C4S_FP32 : r.kind;
+  vector_ok(bias, "bias", r.N);
+  vector_ok(gamma, "gamma", r.K);
+  vector_ok(beta, "beta", r.K);
+  if ((residual && residual->scalar_type() != r.otype) || (out && out->scalar_type() != r.otype))
+    type_error("residual and out must be of the output's type");
+  if (residual) matrix_ok(*residual, "residual", r.M, r.N);
+  if (out) {
+    matrix_ok(*out, "out", r.M, r.N);
+    if (r.M > 1 && out->stride(0) < r.N) value_error("the rows of out must not overlap");
+  }
+  return r;
+}
+
+at::ScalarType dtype_arg(Args& a, const Tensor& x) {   // 0: not given, 1: x's type, 2: fp32
+  switch (a.integer("out_dtype")) {
+    case 0: return at::ScalarType::Undefined;
+    case 1: return x.scalar_type();
+    case 2: return at::kFloat;
+    default: type_error("out is of x's type or fp32");
+  }
+}
+
+// (ctx, device, x, weight, bias, act, residual, layer_norm, gamma, beta, eps, norm_out, out, out_dtype) -> out
+PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args a{args, n};
+    c4s_ctx* ctx = static_cast<c4s_ctx*>(a.pointer("context"));
+    const int dev = (int)a.integer("device");
+    const Tensor &x = a.tensor("x"), &w = a.tensor("weight");
+    const Tensor* bias = a.maybe("bias");
+    const int act = (int)a.integer("act");
+    const Tensor* residual = a.maybe("residual");
+    const bool norm = a.integer("layer_norm") != 0;
+    const Tensor* gamma = a.maybe("gamma");
+    const Tensor* beta = a.maybe("beta");
+    const float eps = (float)a.real("eps");
+    const Tensor* norm_out = a.maybe("norm_out");
+    const Tensor* out = a.maybe("out");
+    const LinCall r = linear_ok(x, w, bias, residual, gamma, beta, out, dtype_arg(a, x));
+    if (norm_out) {
+      matrix_ok(*norm_out, "norm_out", r.M, r.K);
+      if (norm_out->scalar_type() != x.scalar_type() || !norm_out->is_contiguous())
+        value_error("norm_out must be contiguous, of x's type");
+    }
+    on(dev, &x, "x");
+    on(dev, &w, "weight");
+    on(dev, bias, "bias");
+    on(dev, residual, "residual");
+    on(dev, gamma, "gamma");
+    on(dev, beta, "beta");
+    on(dev, norm_out, "norm_out");
+    on(dev, out, "out");
+    Tensor made, scratch;
+    if (!out) {
+      made = at::empty({r.M, r.N}, x.options().dtype(r.otype));
+      out = &made;
+    }
+    if (norm && !norm_out) {
+      scratch = at::empty({r.M, r.K}, x.options());
+      norm_out = &scratch;
+    }
+    auto f = [](const Tensor* t) { return t ? t->const_data_ptr<float>() : nullptr; };
+    const int rc = c4s_linear(ctx, x.const_data_ptr(), r.kind, r.M, r.K, x.stride(0), f(gamma), f(beta), eps,
+                              norm ? norm_out->data_ptr() : nullptr, w.const_data_ptr(), r.N, w.stride(0), f(bias), act,
+                              residual ? residual->const_data_ptr() : nullptr, residual ? residual->stride(0) : 0,
+                              out->data_ptr(), r.okind, out->stride(0), stream_of(dev));
+    if (rc) c_error(ctx, rc, "c4s_linear");
+    return THPVariable_Wrap(*out);
+  });
+}
+
+// (x, weight, bias, residual, gamma, beta, out, out_dtype): the checks alone -> (M, K, N, type of x, of out)
+PyObject* check_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args a{args, n};
+    const Tensor &x = a.tensor("x"), &w = a.tensor("weight");
+    const Tensor* bias = a.maybe("bias");
+    const Tensor* residual = a.maybe("residual");
+    const Tensor* gamma = a.maybe("gamma");
+    const Tensor* beta = a.maybe("beta");
+    const Tensor* out = a.maybe("out");
+    const LinCall r = linear_ok(x, w, bias, residual, gamma, beta, out, dtype_arg(a, x));
+    return Py_BuildValue("iiiii", r.M, r.K, r.N, r.kind, r.okind);
+  });
+}
+
+PyObject* set_error(PyObject*, PyObject* type) {
+  Py_XINCREF(type);
+  Py_XDECREF(g_error);
+  g_error = type;
+  Py_RETURN_NONE;
+}
+
+template <typename F> PyCFunction fast(F f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)); }
+
+PyMethodDef methods[] = {
+    {"kv", fast(kv), METH_FASTCALL, nullptr},
+    {"check_kv", fast(check_kv), METH_FASTCALL, nullptr},
+    {"paged_attention", fast(paged_attention), METH_FASTCALL, nullptr},
+    {"check_attention", fast(check_attention), METH_FASTCALL, nullptr},
+    {"linear", fast(linear), METH_FASTCALL, nullptr},
+    {"check_linear", fast(check_linear), METH_FASTCALL, nullptr},
+    {"set_error", set_error, METH_O, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_c4s", "Binding of the decoder block's operators.", -1, methods,
+                      nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__c4s(void) { return PyModule_Create(&module); }
