@@ -125,15 +125,13 @@ template <typename TO> KvKernel read_kernel(int bits, int cache_dtype) {
 }
 
 using AttnKernel = void (*)(c4s::AttnArgs);
-using JoinKernel = void (*)(c4s::AttnArgs, int);
 struct AttnPick {
-  AttnKernel main = nullptr;
-  JoinKernel join = nullptr;
-  int smem = 0, tok = 0;
+  AttnKernel main = nullptr, join = nullptr;
+  int smem = 0, tok = 0, warps = 0;
 };
 template <typename T, int D, int BITS, int GS, int NQ> AttnPick attn_pick() {
-  using Cfg = c4s::AttnCfg<D, BITS, GS>;
-  return {c4s::attn_kernel<T, D, BITS, GS, NQ>, c4s::attn_join_kernel<T, D, NQ>, Cfg::SMEM, Cfg::TOK};
+  using Cfg = c4s::AttnCfg<D, BITS, GS, NQ>;
+  return {c4s::attn_kernel<T, D, BITS, GS, NQ>, c4s::attn_join_kernel<T, D, NQ>, Cfg::SMEM, Cfg::TOK, Cfg::WARPS};
 }
 template <typename T, int D, int NQ> AttnPick attn_pick_rows(int bits, int group) {
   if (bits == 16) return attn_pick<T, D, 16, 32, NQ>();
@@ -184,11 +182,11 @@ cudaError_t launch_norm(const void* x, int M, int K, int64_t ldx, const float* g
                 eps, (T*)y);
 }
 
-constexpr int ATT_CTAS = 2;                        // per SM: what their shared memory is sized for
-
+// Workspace of the attention: for every warp of the grid two parts of up to 8
+// query heads (six warps a CTA) or 4 (eight warps), and its cut segment.
 int64_t attn_work_bytes(const c4s_ctx* ctx, int dim) {
-  const int64_t W = (int64_t)ctx->num_sms * ATT_CTAS * c4s::ATT_WARPS;
-  return W * 2 * 8 * (dim + 2) * 4;
+  const int64_t ctas = (int64_t)ctx->num_sms * c4s::ATT_CTAS;
+  return ctas * 6 * 2 * 8 * (dim + 2) * 4 + ctas * 8 * (int64_t)sizeof(int4);
 }
 
 }  // namespace
@@ -268,34 +266,41 @@ int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* 
                                     : attn_pick_dim<__half, 8>(cache->head_dim, cache->bits, cache->group));
   cudaError_t e = cudaFuncSetAttribute(k.main, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
   if (e != cudaSuccess) return cuda_fail(ctx, e, "attention kernel attribute");
-  const int ctas = ctx->num_sms * ATT_CTAS;
+  const int ctas = ctx->num_sms * c4s::ATT_CTAS;
+  const int64_t warps = (int64_t)ctas * k.warps;
   c4s::AttnArgs a;
   a.c = view(cache);
   a.table_ld = table_ld;
   a.max_pages = max_pages;
+  a.pdiv = c4s::page_div(cache->page_size);
   a.qb = q_batch_stride;
   a.qh = q_head_stride;
   a.G = G;
   a.scale = scale * 1.4426950408889634f;           // log2(e): the softmax works in powers of two
   a.ob = out_batch_stride;
   a.oh = out_head_stride;
-  a.part_o = static_cast<float*>(d_work);
-  a.part_ml = a.part_o + (size_t)ctas * c4s::ATT_WARPS * 2 * NQ * cache->head_dim;
+  a.cut = static_cast<int4*>(d_work);
+  a.part_o = reinterpret_cast<float*>(a.cut + warps);
+  a.part_ml = a.part_o + warps * 2 * NQ * cache->head_dim;
   a.errflags = ctx->d_err;
-  for (int b0 = 0; b0 < B; b0 += c4s::ATT_MAXB) {
-    a.B = std::min(c4s::ATT_MAXB, B - b0);
+  // tiles that the page table can name: a launch's prefix sums of them stay inside 32 bits
+  const long long cap = std::min<long long>((long long)max_pages * cache->page_size, 0x7fffffffLL);
+  const long long cap_tiles = c4s::kv_tiles(0, cap, k.tok);
+  const int group = (int)std::min<long long>(c4s::ATT_MAXB, 0x7fffffffLL / cap_tiles);
+  const int passes = (G + NQ - 1) / NQ;
+  for (int b0 = 0; b0 < B; b0 += group) {
+    a.B = std::min(group, B - b0);
     a.table = d_page_table + (int64_t)b0 * table_ld;
     a.q = static_cast<const unsigned short*>(d_q) + (int64_t)b0 * q_batch_stride;
     a.out = static_cast<unsigned short*>(d_out) + (int64_t)b0 * out_batch_stride;
     a.len = d_len + b0;
     a.start = d_start ? d_start + b0 : nullptr;
-    // no more warps than there can be tiles
-    const long long most = (long long)a.B * c4s::kv_tiles(0, (long long)max_pages * cache->page_size, k.tok) *
-                           cache->kv_heads * ((G + NQ - 1) / NQ);
-    const int grid = (int)std::min<long long>(ctas, (most + c4s::ATT_WARPS - 1) / c4s::ATT_WARPS);
-    e = launch(k.main, dim3((unsigned)grid), 32 * c4s::ATT_WARPS, k.smem, stream, a);
+    // no more CTAs than there can be tiles for their first warps
+    const long long most = a.B * cap_tiles * cache->kv_heads * passes;
+    const int grid = (int)std::min<long long>(ctas, most);
+    e = launch(k.main, dim3((unsigned)grid), 32 * k.warps, k.smem, stream, a);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "attention launch");
-    e = launch(k.join, dim3((unsigned)(grid * c4s::ATT_WARPS)), 32 * c4s::ATT_WARPS, 0, stream, a, k.tok);
+    e = launch(k.join, dim3((unsigned)(grid * k.warps), (unsigned)std::min(G, NQ)), c4s::ATT_JOIN_NT, 0, stream, a);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "attention join launch");
   }
   return C4S_OK;

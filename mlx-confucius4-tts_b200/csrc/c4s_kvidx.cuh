@@ -35,6 +35,21 @@ C4S_HD bool kv_locate(const int* table_row, int max_pages, int num_pages, int pa
   return true;
 }
 
+// Division by a page size d in a loop: for 0 <= n < 2^31 and d >= 1, with
+// s = ceil(log2 d) and m = floor(2^(31+s) / d) + 1 (at most 2^32), n / d is
+// n m >> (31 + s): m d = 2^(31+s) + e with 0 < e <= d <= 2^s, so n m / 2^(31+s)
+// exceeds n / d by n e / (d 2^(31+s)) < 1 / d.
+struct PageDiv {
+  unsigned long long mul;
+  int shift;
+};
+C4S_HD PageDiv page_div(int d) {
+  int s = 0;
+  while (s < 31 && (1LL << s) < d) ++s;
+  return {((1ULL << (31 + s)) / (unsigned)d) + 1, 31 + s};
+}
+C4S_HD int page_of(const PageDiv& p, int n) { return (int)(((unsigned long long)(unsigned)n * p.mul) >> p.shift); }
+
 // The visible positions [lo, hi) of a sequence: its length, cut to what the
 // page table can name, from its first visible position on.
 C4S_HD void kv_visible(int len, int start, int max_pages, int page_size, long long& lo, long long& hi) {
@@ -59,7 +74,8 @@ C4S_HD int split_owner(long long T, int W, long long tile) {
 
 // Largest b in [0, B) with P[b] <= x, for 0 <= x < P[B]: the sequence of tile
 // x * HB + anything. Sequences without tiles (P[b] == P[b + 1]) are passed over.
-C4S_HD int split_sequence(const long long* P, int B, long long x) {
+template <typename I>
+C4S_HD int split_sequence(const I* P, int B, long long x) {
   int a = 0, e = B;
   while (e - a > 1) {
     const int m = (a + e) >> 1;

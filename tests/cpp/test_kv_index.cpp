@@ -37,6 +37,15 @@ int main() {
     big[2] = 9;
     CHECK(kv_locate(big.data(), 3, 10, 1500000000, 3000000001LL, pg, sl) && pg == 9 && sl == 1);
   }
+  // the loop's division
+  for (int it = 0; it < 300000; ++it) {
+    const int d = it < 3000 ? it + 1 : 1 + (int)(r() % (it % 2 ? 70000u : 0x7fffffffu));
+    const PageDiv p = page_div(d);
+    CHECK(p.mul <= (1ULL << 32));
+    const int edge = (int)((r() % (0x80000000ULL / d)) * d);
+    for (int n : {0, 1, d - 1, edge, edge > 0 ? edge - 1 : 0, (int)(r() & 0x7fffffff), 0x7fffffff, 0x7ffffffe})
+      CHECK(page_of(p, n) == n / d);
+  }
   // visible ranges
   {
     long long lo, hi;
