@@ -70,7 +70,7 @@ template <int D, int BITS, int GS, int NQ>
 struct AttnCfg {
   static constexpr int ROW = D * BITS / 8;                     // bytes of a cache row
   static constexpr int NG = BITS == 16 ? 1 : D / GS;           // quantization groups of a row
-  static constexpr int TOK = ROW <= 96 ? 32 : 16;              // tokens per tile
+  static constexpr int TOK = ROW <= (BITS == 16 ? 128 : 96) ? 32 : 16;              // tokens per tile
   static constexpr int PITCH = BITS == 16 && ROW % 128 ? ROW + 16 : ROW;
   static constexpr int CH = ROW / 16;                          // 16-byte chunks per row
   static constexpr int STAGE = 2 * TOK * (PITCH + (BITS == 16 ? 0 : 8 * NG));   // bytes: keys, values, their scales
