@@ -165,7 +165,9 @@ struct TilePick {
   TileKernel kern;
   size_t smem;
 };
+// bn 64, 128: one CTA a tile; 256: pairs of CTAs
 template <typename TI, typename TO> TilePick tile_pick(int bn) {
+  if (bn == 256) return TilePick{c4s::lin_pair_kernel<TI, TO>, c4s::LP_SMEM};
   return bn == 64 ? TilePick{c4s::lin_tile_kernel<TI, TO, 64>, c4s::LinCfg<64>::SMEM}
                   : TilePick{c4s::lin_tile_kernel<TI, TO, 128>, c4s::LinCfg<128>::SMEM};
 }
@@ -344,16 +346,19 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
     d_x = d_norm;
     ld_x = K;
   }
-  // tiles of 128 columns where they fill the machine, else of 64, and clusters that share a tile's K
+  // pairs of CTAs on 256 x 256 tiles where those fill the machine; else tiles of 128 columns where they do,
+  // else of 64, and clusters that share a tile's K
   const int mt = (M + c4s::LN_BM - 1) / c4s::LN_BM, KB = (K + c4s::LN_BK - 1) / c4s::LN_BK;
-  const int bn = (long long)mt * ((N + 127) / 128) >= ctx->num_sms ? 128 : 64;
+  const long long big = (long long)((M + 255) / 256) * ((N + 255) / 256);
+  const bool pair = big * 2 >= ctx->num_sms;
+  const int bn = pair ? 256 : (long long)mt * ((N + 127) / 128) >= ctx->num_sms ? 128 : 64;
   const long long nt = (N + bn - 1) / bn;
   int S = 1;
-  while (S < 8 && nt * mt * S * 2 <= ctx->num_sms + ctx->num_sms / 4 && KB >= S * 2 * 4) S *= 2;
-  const int box = std::min(c4s::LN_BM, (M + 7) / 8 * 8);
+  while (!pair && S < 8 && nt * mt * S * 2 <= ctx->num_sms + ctx->num_sms / 4 && KB >= S * 2 * 4) S *= 2;
+  const int box = pair ? c4s::LN_BM : std::min(c4s::LN_BM, (M + 7) / 8 * 8);
   CUtensorMap tx, tw;
   if (!encode_rows(&tx, dtype, d_x, K, M, ld_x * 2, box) ||
-      !encode_rows(&tw, dtype, d_weight, K, N, ld_weight * 2, bn))
+      !encode_rows(&tw, dtype, d_weight, K, N, ld_weight * 2, pair ? 128 : bn))
     return fail(ctx, C4S_ERR_CUDA, "tensor map encoding failed");
   c4s::LinArgs a;
   a.bias = d_bias;
@@ -375,7 +380,8 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
   e = cudaFuncSetAttribute(k.kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem);
   if (e != cudaSuccess) return cuda_fail(ctx, e, "linear kernel attribute");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(nt * S), (unsigned)mt);
+  const int cluster = pair ? 2 : S;
+  cfg.gridDim = pair ? dim3((unsigned)(2 * std::min<long long>(big, ctx->num_sms / 2))) : dim3((unsigned)(nt * S), (unsigned)mt);
   cfg.blockDim = dim3(c4s::LN_THREADS);
   cfg.dynamicSmemBytes = k.smem;
   cfg.stream = (cudaStream_t)stream;
@@ -383,11 +389,11 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = (unsigned)S;
+  at[1].val.clusterDim.x = (unsigned)cluster;
   at[1].val.clusterDim.y = 1;
   at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = S > 1 ? 2 : 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, k.kern, tx, tw, a, S);
   return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "linear launch");
 } catch (...) {

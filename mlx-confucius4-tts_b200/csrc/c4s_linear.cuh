@@ -13,6 +13,7 @@
 // tiles are fewer than the SMs, a cluster of S CTAs shares a tile: each takes
 // a part of K, leaves its fp32 partial in its own shared memory, and sums a
 // share of the rows over the cluster in a fixed order.
+// lin_pair_kernel: 256 x 256 tiles by pairs of CTAs, for large products.
 #pragma once
 
 #include "c4s_tc.cuh"
@@ -38,68 +39,101 @@ struct LinArgs {
   unsigned* errflags;
 };
 
-__device__ __forceinline__ float activate(float x, int act) {
-  switch (act) {
-    case C4S_ACT_GELU: {
+// The activation of N values; one branch for all of them.
+template <int N>
+__device__ __forceinline__ void activate(float (&x)[N], int act) {
+  if (act == C4S_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
       // 0.5 x (1 + tanh u) = x / (1 + e^(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
-      const float u = 0.7978845608028654f * fmaf(0.044715f * x, x * x, x);
-      return x / (1.0f + __expf(-2.0f * u));
+      const float u = 0.7978845608028654f * fmaf(0.044715f * x[i], x[i] * x[i], x[i]);
+      x[i] = __fdividef(x[i], 1.0f + __expf(-2.0f * u));
     }
-    case C4S_ACT_GELU_ERF: return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
-    case C4S_ACT_SILU: return x / (1.0f + __expf(-x));
-    case C4S_ACT_RELU: return x < 0.0f ? 0.0f : x;   // NaN stays
-    default: return x;
+  } else if (act == C4S_ACT_GELU_ERF) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = 0.5f * x[i] * (1.0f + erff(x[i] * 0.70710678118654752f));
+  } else if (act == C4S_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __fdividef(x[i], 1.0f + __expf(-x[i]));
+  } else if (act == C4S_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = x[i] < 0.0f ? 0.0f : x[i];   // NaN stays
   }
 }
 
-// NV consecutive outputs of a row from column n: residual, rounding, store.
+// NV consecutive columns of bias from column n (zeros past N).
+template <int NV>
+__device__ __forceinline__ void lin_bias(const LinArgs& a, int n, float (&b)[NV]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) b[i] = a.bias && n + i < a.N ? __ldg(a.bias + n + i) : 0.0f;
+}
+
+// NV consecutive outputs of a row from column n, given their sums of products:
+// bias, activation, residual, rounding, store.
 template <typename TO, int NV>
-__device__ __forceinline__ void lin_store(const LinArgs& a, long long row, int n, float (&v)[NV]) {
+__device__ __forceinline__ void lin_store(const LinArgs& a, long long row, int n, float (&v)[NV], const float (&b)[NV]) {
   static_assert(NV * sizeof(TO) == 16, "one 16-byte store");
   TO* o = static_cast<TO*>(a.out) + row * a.ldo + n;
   const bool full = n + NV <= a.N;
+  __align__(16) TO x[NV];
   if (a.residual) {
     const TO* r = static_cast<const TO*>(a.residual) + row * a.ldr + n;
     if (full && a.vec_res) {
-      TO x[NV];
       *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(r);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) v[i] += Cvt<TO>::f(x[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (n + i < a.N) v[i] += Cvt<TO>::f(r[i]);
+      for (int i = 0; i < NV; ++i) x[i] = n + i < a.N ? r[i] : Cvt<TO>::t(0.0f);
     }
   }
-  if (full && a.vec_out) {
-    __align__(16) TO x[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = Cvt<TO>::t(v[i]);
+  for (int i = 0; i < NV; ++i) v[i] += b[i];
+  activate(v, a.act);
+  if (a.residual)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] += Cvt<TO>::f(x[i]);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) x[i] = Cvt<TO>::t(v[i]);
+  if (full && a.vec_out) {
     *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(x);
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (n + i < a.N) o[i] = Cvt<TO>::t(v[i]);
+      if (n + i < a.N) o[i] = x[i];
   }
 }
 
-// A warp's 32 x 32 block of finished values (fp32, row pitch LN_STAGE_PITCH)
-// to the output: NV columns a lane, whole 16-byte pieces of rows.
+// A warp's 32 x 32 block of the accumulator (TMEM lanes of its quarter, from
+// column tcol) to the output at row m0, column n0: lane = row on the way out of
+// TMEM, through the warp's staging block, then whole 16-byte pieces of rows.
 template <typename TO>
-__device__ __forceinline__ void lin_store_block(const LinArgs& a, const float* st, long long m0, int n0, int lane) {
+__device__ __forceinline__ void lin_block(const LinArgs& a, unsigned taddr, float* st, long long m0, int n0, int lane) {
   constexpr int NV = 16 / sizeof(TO), LPR = 32 / NV, RPI = 32 / LPR;   // lanes per row, rows per pass
   const int c = (lane % LPR) * NV;
+  float b[NV];
+  lin_bias(a, n0 + c, b);
+  {
+    unsigned r[32];
+    tmem_ld32(taddr, r);
+    tmem_ld_wait();
 #pragma unroll
-  for (int i = 0; i < 32 / RPI; ++i) {
-    const int r = i * RPI + lane / LPR;
-    if (m0 + r < a.M && n0 + c < a.N) {
+    for (int j = 0; j < 32; j += 4)
+      *reinterpret_cast<float4*>(st + lane * LN_STAGE_PITCH + j) =
+          make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+  }
+  __syncwarp();
+  if (n0 + c < a.N) {
+#pragma unroll 2
+    for (int i = 0; i < 32 / RPI; ++i) {
+      const int r = i * RPI + lane / LPR;
+      if (m0 + r >= a.M) break;
       float v[NV];
 #pragma unroll
       for (int j = 0; j < NV; j += 4)
         *reinterpret_cast<float4*>(&v[j]) = *reinterpret_cast<const float4*>(st + r * LN_STAGE_PITCH + c + j);
-      lin_store<TO, NV>(a, m0 + r, n0 + c, v);
+      lin_store<TO, NV>(a, m0 + r, n0 + c, v, b);
     }
   }
+  __syncwarp();
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -205,27 +239,15 @@ __global__ void __launch_bounds__(LN_THREADS, 1) lin_tile_kernel(const __grid_co
     const int rows = min(LN_BM, a.M - m0);
     if (ok && !abort_flag && k1 > k0 && 32 * q < rows) {
       for (int c = half; c < BN / 32; c += 2) {
-        unsigned r[32];
-        tmem_ld32(tmem + ((unsigned)(32 * q) << 16) + (unsigned)(32 * c), r);
-        tmem_ld_wait();
+        const unsigned taddr = tmem + ((unsigned)(32 * q) << 16) + (unsigned)(32 * c);
         if (S == 1) {
-          // lane = row: bias and activation, through the warp's staging block (in the idle ring) to whole rows
-          float* st = reinterpret_cast<float*>(ring) + (warp - 2) * 32 * LN_STAGE_PITCH;
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            float4 v;
-            float* pv = &v.x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int n = n0 + 32 * c + j + e;
-              pv[e] = activate(__uint_as_float(r[j + e]) + (a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f), a.act);
-            }
-            *reinterpret_cast<float4*>(st + lane * LN_STAGE_PITCH + j) = v;
-          }
-          __syncwarp();
-          lin_store_block<TO>(a, st, (long long)m0 + 32 * q, n0 + 32 * c, lane);
-          __syncwarp();
+          // staging blocks in the idle ring: every copy has landed and been read
+          lin_block<TO>(a, taddr, reinterpret_cast<float*>(ring) + (warp - 2) * 32 * LN_STAGE_PITCH,
+                        (long long)m0 + 32 * q, n0 + 32 * c, lane);
         } else {
+          unsigned r[32];
+          tmem_ld32(taddr, r);
+          tmem_ld_wait();
           float* p = reinterpret_cast<float*>(ring) + (32 * q + lane) * Cfg::PPITCH + 32 * c;
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
@@ -247,34 +269,197 @@ __global__ void __launch_bounds__(LN_THREADS, 1) lin_tile_kernel(const __grid_co
     cluster_wait();
     const int rows = min(LN_BM, a.M - m0);
     const int r0 = rows * s / S, r1 = rows * (s + 1) / S;     // this CTA's share of the rows
-    constexpr int CG = BN / 4;                                // 4 columns a thread
+    constexpr int NV = 16 / sizeof(TO), CG = BN / NV;         // NV columns a thread
     if (!abort_flag) {
       for (int i = threadIdx.x; i < (r1 - r0) * CG; i += LN_THREADS) {
-        const int r = r0 + i / CG, c = (i % CG) * 4;
+        const int r = r0 + i / CG, c = (i % CG) * NV;
         if (n0 + c >= a.N) continue;
-        const unsigned addr = smem_u32(ring) + (unsigned)(r * Cfg::PPITCH + c) * 4u;
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int p = 0; p < S; ++p) {
-          const float4 x = ld_cluster(addr, (unsigned)p);
-          v[0] += x.x;
-          v[1] += x.y;
-          v[2] += x.z;
-          v[3] += x.w;
-        }
-        const long long row = (long long)m0 + r;
+        float v[NV], b[NV];
+        lin_bias(a, n0 + c, b);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = n0 + c + e;
-          if (n >= a.N) break;
-          float y = activate(v[e] + (a.bias ? __ldg(a.bias + n) : 0.0f), a.act);
-          if (a.residual) y += Cvt<TO>::f(static_cast<const TO*>(a.residual)[row * a.ldr + n]);
-          static_cast<TO*>(a.out)[row * a.ldo + n] = Cvt<TO>::t(y);
-        }
+        for (int j = 0; j < NV; ++j) v[j] = 0.0f;
+        const unsigned addr = smem_u32(ring) + (unsigned)(r * Cfg::PPITCH + c) * 4u;
+        for (int p = 0; p < S; ++p)
+#pragma unroll
+          for (int j = 0; j < NV; j += 4) {
+            const float4 x = ld_cluster(addr + 4u * j, (unsigned)p);
+            v[j] += x.x;
+            v[j + 1] += x.y;
+            v[j + 2] += x.z;
+            v[j + 3] += x.w;
+          }
+        lin_store<TO, NV>(a, (long long)m0 + r, n0 + c, v, b);
       }
     }
     cluster_arrive();
     cluster_wait();                                // no CTA leaves while another reads its partial
   }
+}
+
+// ---- large products: pairs of SMs on 256 x 256 tiles ------------------------
+// One 128 x 128 tile per CTA needs 32 KB from L2 for 256 cycles of products,
+// more than an SM gets. A pair of CTAs (cta_group::2) works a 256 x 256 tile:
+// each holds 128 rows of x and 128 rows of W per k-block and reads the other's
+// half through the pair, half the bytes per product. Persistent: the pairs
+// take tiles in turn, the accumulator is double-buffered in TMEM (2 x 256
+// columns), and the eight epilogue warps of each CTA finish a tile while the
+// next one's products run.
+constexpr int LP_ST = 5;                           // stages of the ring
+constexpr unsigned LP_HALF = 128 * LN_BK * 2;      // 16 KB: a CTA's rows of x, or of W, of one k-block
+constexpr size_t LP_STAGING = (size_t)LN_EPI_WARPS * 32 * LN_STAGE_PITCH * 4;
+constexpr size_t LP_SMEM = LP_ST * 2 * (size_t)LP_HALF + LP_STAGING + 1024;
+
+__device__ __forceinline__ unsigned map_rank(unsigned addr, unsigned rank) {
+  unsigned p;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
+  return p;
+}
+// A tile into this CTA's memory, counted on a barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, unsigned bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void umma_pair(unsigned tmem_d, unsigned long long adesc, unsigned long long bdesc,
+                                          unsigned idesc, unsigned accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs once the products issued so far are done.
+__device__ __forceinline__ void umma_commit_pair(unsigned long long* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((unsigned short)3)
+      : "memory");
+}
+
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(LN_THREADS, 1) lin_pair_kernel(const __grid_constant__ CUtensorMap tmX,
+                                                                 const __grid_constant__ CUtensorMap tmW, LinArgs a,
+                                                                 int) {
+  constexpr unsigned BF = std::is_same<TI, __nv_bfloat16>::value ? 1u : 0u;
+  constexpr unsigned IDESC = (1u << 4) | (BF << 7) | (BF << 10) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+  extern __shared__ unsigned char lsm_raw[];
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<unsigned long long>(lsm_raw) + 1023ull) & ~1023ull);
+  float* staging = reinterpret_cast<float*>(ring + LP_ST * 2 * (size_t)LP_HALF);
+  __shared__ unsigned long long full[LP_ST], empty[LP_ST], acc_full[2], acc_empty[2];
+  __shared__ unsigned tmem_base;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned rank = blockIdx.x & 1u;           // in the pair
+  const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+  const int KB = (a.K + LN_BK - 1) / LN_BK;
+  const int mt = (a.M + 255) / 256, nt = (a.N + 255) / 256;
+  const long long tiles = (long long)mt * nt;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < LP_ST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 2 * LN_EPI_WARPS);  // both CTAs' epilogue warps
+    }
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  tc_fence_after();
+  const unsigned tmem = tmem_base;
+  grid_dep_wait();
+  grid_dep_launch();
+  auto give_up = [&]() {
+    atomicOr(a.errflags, C4S_DEVERR_TIMEOUT);
+    abort_flag = 1;
+  };
+  if (warp == 0) {
+    if (lane == 0) {
+      // both CTAs copy their halves; the first CTA's barrier counts the bytes of both
+      int it = 0;
+      for (long long t = pair; t < tiles && !abort_flag; t += pairs) {
+        const int m0 = (int)(t % mt) * 256 + (int)rank * 128, n0 = (int)(t / mt) * 256 + (int)rank * 128;
+        for (int kb = 0; kb < KB && !abort_flag; ++kb, ++it) {
+          const int i = it % LP_ST;
+          if (!mbar_wait_1s(&empty[i], ((unsigned)(it / LP_ST) & 1u) ^ 1u)) { give_up(); break; }
+          unsigned char* sx = ring + (size_t)i * 2 * LP_HALF;
+          const unsigned bar = map_rank(smem_u32(&full[i]), 0u);
+          if (rank == 0) mbar_arrive_expect_tx(&full[i], 4 * LP_HALF);
+          tma_load_pair(sx, &tmX, kb * LN_BK, m0, bar);
+          tma_load_pair(sx + LP_HALF, &tmW, kb * LN_BK, n0, bar);
+        }
+      }
+      // after a wait that gave up: the copies in flight land before the pair goes
+      if (abort_flag && rank == 0)
+        for (int j = max(0, it - LP_ST); j < it; ++j) mbar_wait_1s(&full[j % LP_ST], (unsigned)(j / LP_ST) & 1u);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int it = 0, n = 0;
+      for (long long t = pair; t < tiles && !abort_flag; t += pairs, ++n) {
+        const int buf = n & 1;
+        if (!mbar_wait_1s(&acc_empty[buf], ((unsigned)(n >> 1) & 1u) ^ 1u)) { give_up(); break; }
+        tc_fence_after();
+        for (int kb = 0; kb < KB && !abort_flag; ++kb, ++it) {
+          const int i = it % LP_ST;
+          if (!mbar_wait_1s(&full[i], (unsigned)(it / LP_ST) & 1u)) { give_up(); break; }
+          tc_fence_after();
+          const unsigned char* sx = ring + (size_t)i * 2 * LP_HALF;
+          const unsigned long long xd = sw128_desc(sx), wd = sw128_desc(sx + LP_HALF);
+#pragma unroll
+          for (int kk = 0; kk < LN_BK / 16; ++kk)
+            umma_pair(tmem + (unsigned)(buf * 256), xd + 2ull * kk, wd + 2ull * kk, IDESC, (kb | kk) != 0 ? 1u : 0u);
+          umma_commit_pair(&empty[i]);
+        }
+        umma_commit_pair(&acc_full[buf]);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    float* st = staging + (warp - 2) * 32 * LN_STAGE_PITCH;
+    int n = 0;
+    for (long long t = pair; t < tiles; t += pairs, ++n) {
+      const int buf = n & 1;
+      const long long m0 = (t % mt) * 256 + rank * 128 + 32 * q;
+      const int n0 = (int)(t / mt) * 256;
+      const bool ok = mbar_wait_1s(&acc_full[buf], (unsigned)(n >> 1) & 1u);
+      if (!ok) give_up();
+      tc_fence_after();
+      if (!__all_sync(FULL, ok) || abort_flag) break;
+      if (m0 < a.M)
+        for (int c = 4 * half; c < 4 * half + 4 && n0 + 32 * c < a.N; ++c)
+          lin_block<TO>(a, tmem + ((unsigned)(32 * q) << 16) + (unsigned)(buf * 256 + 32 * c), st, m0, n0 + 32 * c, lane);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        const unsigned bar = map_rank(smem_u32(&acc_empty[buf]), 0u);
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();                                  // the pair's products and copies are done on both sides
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // LayerNorm of the rows (nn.cpp:73-83: biased variance, (x - mean) / sqrt(var

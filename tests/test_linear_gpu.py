@@ -77,7 +77,8 @@ def operands(M, K, N, dtype, g):
 
 SHAPES = [(1, 1280, 3840), (1, 5120, 1280), (2, 8, 1), (3, 64, 65), (5, 200, 129), (8, 1280, 5120), (9, 5120, 640),
           (16, 1272, 77), (17, 320, 1280), (64, 5120, 1280), (65, 1280, 1000), (128, 2048, 256), (200, 72, 3333),
-          (256, 1280, 5120), (300, 4104, 130), (1000, 640, 2000), (2049, 1280, 1281)]
+          (256, 1280, 5120), (300, 4104, 130), (1000, 640, 2000), (2049, 1280, 1281), (4100, 200, 1300),
+          (2305, 1280, 5160)]
 
 
 @pytest.mark.parametrize("dtype,odt", [(BF, BF), (FP, FP), (BF, F32), (FP, F32)])
