@@ -176,12 +176,27 @@ template <typename T>
 cudaError_t launch_norm(const void* x, int M, int K, int64_t ldx, const float* gamma, const float* beta, float eps,
                         void* y, void* stream) {
   const bool vec = ((uintptr_t)x & 15) == 0 && (ldx & 7) == 0;
-  const int vpt = (K / 8 + c4s::LNORM_NT - 1) / c4s::LNORM_NT;
-  auto kern = vpt <= 1 ? c4s::lin_norm_kernel<T, 1>
-              : vpt <= 2 ? c4s::lin_norm_kernel<T, 2>
-              : vpt <= 4 ? c4s::lin_norm_kernel<T, 4> : c4s::lin_norm_kernel<T, 8>;
-  return launch(kern, dim3((unsigned)M), c4s::LNORM_NT, 0, stream, (const T*)x, (long long)ldx, K, vec, gamma, beta,
-                eps, (T*)y);
+  // a warp per row up to 2048 columns, else a CTA per row
+  const int vec_n = K / 8, wide = vec_n > 8 * 32, rows = wide ? 1 : c4s::LNORM_NT / 32;
+  const int vpt = (vec_n + (wide ? c4s::LNORM_NT : 32) - 1) / (wide ? c4s::LNORM_NT : 32);
+  auto kern = wide ? (vpt <= 4 ? c4s::lin_norm_kernel<T, 4, 128> : c4s::lin_norm_kernel<T, 8, 128>)
+              : vpt <= 2 ? c4s::lin_norm_kernel<T, 2, 32>
+              : vpt <= 5 ? c4s::lin_norm_kernel<T, 5, 32> : c4s::lin_norm_kernel<T, 8, 32>;
+  return launch(kern, dim3((unsigned)((M + rows - 1) / rows)), c4s::LNORM_NT, 0, stream, (const T*)x, (long long)ldx, M,
+                K, vec, gamma, beta, eps, (T*)y);
+}
+
+// The kernel for few rows (M <= 16).
+template <typename TI, typename TO>
+cudaError_t launch_few(const c4s_ctx* ctx, const void* x, long long ldx, const float* gamma, const float* beta, float eps,
+                       bool norm, const void* w, long long ldw, const c4s::LinArgs& a, void* stream) {
+  const bool xvec = ((uintptr_t)x & 15) == 0 && (ldx & 7) == 0;
+  const bool r16 = a.N >= 16 * ctx->num_sms;
+  auto kern = a.M <= 8 ? (r16 ? c4s::lin_few_kernel<TI, TO, 16, 1> : c4s::lin_few_kernel<TI, TO, 8, 1>)
+                       : (r16 ? c4s::lin_few_kernel<TI, TO, 16, 2> : c4s::lin_few_kernel<TI, TO, 8, 2>);
+  const int R = r16 ? 16 : 8;
+  return launch(kern, dim3((unsigned)((a.N + R - 1) / R)), 32 * c4s::LF_WARPS, 0, stream, (const TI*)x, ldx, xvec, gamma,
+                beta, eps, norm, (const TI*)w, ldw, a);
 }
 
 // Workspace of the attention: for every warp of the grid two parts of up to 8
@@ -339,6 +354,29 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
   DeviceGuard dg(ctx->device);
   if (!dg.ok) return fail(ctx, C4S_ERR_CUDA, "cannot select the context's device");
   cudaError_t e;
+  c4s::LinArgs a;
+  a.bias = d_bias;
+  a.residual = d_residual;
+  a.ldr = ld_residual;
+  a.out = d_out;
+  a.ldo = ld_out;
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.act = act;
+  a.vec_out = ((uintptr_t)d_out & 15) == 0 && (ld_out * os) % 16 == 0;
+  a.vec_res = ((uintptr_t)d_residual & 15) == 0 && (ld_residual * os) % 16 == 0;
+  a.errflags = ctx->d_err;
+  a.xbytes = 0;
+  if (M <= 16) {
+    const bool f32 = out_dtype == C4S_FP32, norm = d_norm != nullptr;
+    e = dtype == C4S_BF16
+            ? (f32 ? launch_few<__nv_bfloat16, float>(ctx, d_x, ld_x, d_gamma, d_beta, eps, norm, d_weight, ld_weight, a, stream)
+                   : launch_few<__nv_bfloat16, __nv_bfloat16>(ctx, d_x, ld_x, d_gamma, d_beta, eps, norm, d_weight, ld_weight, a, stream))
+            : (f32 ? launch_few<__half, float>(ctx, d_x, ld_x, d_gamma, d_beta, eps, norm, d_weight, ld_weight, a, stream)
+                   : launch_few<__half, __half>(ctx, d_x, ld_x, d_gamma, d_beta, eps, norm, d_weight, ld_weight, a, stream));
+    return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "linear launch");
+  }
   if (d_norm) {
     e = dtype == C4S_BF16 ? launch_norm<__nv_bfloat16>(d_x, M, K, ld_x, d_gamma, d_beta, eps, d_norm, stream)
                           : launch_norm<__half>(d_x, M, K, ld_x, d_gamma, d_beta, eps, d_norm, stream);
@@ -360,20 +398,7 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
   if (!encode_rows(&tx, dtype, d_x, K, M, ld_x * 2, box) ||
       !encode_rows(&tw, dtype, d_weight, K, N, ld_weight * 2, pair ? 128 : bn))
     return fail(ctx, C4S_ERR_CUDA, "tensor map encoding failed");
-  c4s::LinArgs a;
-  a.bias = d_bias;
-  a.residual = d_residual;
-  a.ldr = ld_residual;
-  a.out = d_out;
-  a.ldo = ld_out;
-  a.M = M;
-  a.N = N;
-  a.K = K;
-  a.act = act;
-  a.vec_out = ((uintptr_t)d_out & 15) == 0 && (ld_out * os) % 16 == 0;
-  a.vec_res = ((uintptr_t)d_residual & 15) == 0 && (ld_residual * os) % 16 == 0;
   a.xbytes = (unsigned)box * c4s::LN_BK * 2;
-  a.errflags = ctx->d_err;
   const TilePick k = dtype == C4S_BF16
                          ? (out_dtype == C4S_FP32 ? tile_pick<__nv_bfloat16, float>(bn) : tile_pick<__nv_bfloat16, __nv_bfloat16>(bn))
                          : (out_dtype == C4S_FP32 ? tile_pick<__half, float>(bn) : tile_pick<__half, __half>(bn));

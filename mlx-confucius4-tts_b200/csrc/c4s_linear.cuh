@@ -14,6 +14,7 @@
 // a part of K, leaves its fp32 partial in its own shared memory, and sums a
 // share of the rows over the cluster in a fixed order.
 // lin_pair_kernel: 256 x 256 tiles by pairs of CTAs, for large products.
+// lin_few_kernel: few rows of x, the weight streamed once, no TMEM.
 #pragma once
 
 #include "c4s_tc.cuh"
@@ -22,9 +23,30 @@ namespace c4s {
 
 constexpr int LN_BM = 128, LN_BK = 64;
 constexpr int LN_EPI_WARPS = 8;
+constexpr int LN_MAX_SPLIT = 8;                    // CTAs that share a tile's K
 constexpr int LN_THREADS = 64 + 32 * LN_EPI_WARPS;
 constexpr int LN_STAGE_PITCH = 36;                 // floats per row of a warp's 32 x 32 staging block (16-byte rows,
                                                    // eight rows on different banks)
+
+// 8 consecutive elements of a row that several CTAs read.
+template <typename T>
+__device__ __forceinline__ void load8c(const T* p, bool vec, T (&x)[8]) {
+  if (vec) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    memcpy(x, &w, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p[i];
+  }
+}
+// The norm's scale and shift of 8 consecutive columns (k a multiple of 8).
+__device__ __forceinline__ void lin_gamma(const float* gamma, const float* beta, int k, float (&ga)[8], float (&be)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    ga[i] = gamma ? __ldg(gamma + k + i) : 1.0f;
+    be[i] = beta ? __ldg(beta + k + i) : 0.0f;
+  }
+}
 
 struct LinArgs {
   const float* bias;                               // [N] or null
@@ -147,10 +169,17 @@ __device__ __forceinline__ float4 ld_cluster(unsigned addr, unsigned rank) {
   return v;
 }
 
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
+                   reinterpret_cast<unsigned long long>(map)),
+               "r"(x), "r"(y)
+               : "memory");
+}
+
 template <int BN>
 struct LinCfg {
   static constexpr unsigned XB = LN_BM * LN_BK * 2, WB = BN * LN_BK * 2;   // bytes of a stage's tiles
-  static constexpr int STAGES = BN <= 64 ? 8 : 6;
+  static constexpr int STAGES = BN <= 64 ? 4 : 6;                           // 64: two CTAs per SM
   static constexpr int PPITCH = BN + 4;                                    // floats per row of a split tile's partial
   static constexpr size_t SMEM = STAGES * (size_t)(XB + WB) + 1024;
   static_assert((size_t)LN_BM * PPITCH * 4 <= STAGES * (size_t)(XB + WB), "the partial fits the ring");
@@ -159,7 +188,7 @@ struct LinCfg {
 
 // TI: operands; TO: output; grid (ceil(N / BN) S, ceil(M / 128)), clusters of S along x.
 template <typename TI, typename TO, int BN>
-__global__ void __launch_bounds__(LN_THREADS, 1) lin_tile_kernel(const __grid_constant__ CUtensorMap tmX,
+__global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(const __grid_constant__ CUtensorMap tmX,
                                                                  const __grid_constant__ CUtensorMap tmW, LinArgs a,
                                                                  int S) {
   using Cfg = LinCfg<BN>;
@@ -192,6 +221,8 @@ __global__ void __launch_bounds__(LN_THREADS, 1) lin_tile_kernel(const __grid_co
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = tmem_base;
+  // the weight's tiles on their way to L2 while the kernel before this one still runs
+  if (warp == 0 && lane < k1 - k0) tma_prefetch_2d(&tmW, (k0 + lane) * LN_BK, n0);
   grid_dep_wait();                                 // x (the norm's output among it) and the residual
   grid_dep_launch();
   auto give_up = [&]() {
@@ -279,15 +310,20 @@ __global__ void __launch_bounds__(LN_THREADS, 1) lin_tile_kernel(const __grid_co
 #pragma unroll
         for (int j = 0; j < NV; ++j) v[j] = 0.0f;
         const unsigned addr = smem_u32(ring) + (unsigned)(r * Cfg::PPITCH + c) * 4u;
-        for (int p = 0; p < S; ++p)
 #pragma unroll
-          for (int j = 0; j < NV; j += 4) {
-            const float4 x = ld_cluster(addr + 4u * j, (unsigned)p);
-            v[j] += x.x;
-            v[j + 1] += x.y;
-            v[j + 2] += x.z;
-            v[j + 3] += x.w;
+        for (int j = 0; j < NV; j += 4) {
+          float4 x[LN_MAX_SPLIT];                  // all on their way before any is added
+#pragma unroll
+          for (int p = 0; p < LN_MAX_SPLIT; ++p)
+            x[p] = p < S ? ld_cluster(addr + 4u * j, (unsigned)p) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int p = 0; p < LN_MAX_SPLIT; ++p) {
+            v[j] += x[p].x;
+            v[j + 1] += x[p].y;
+            v[j + 2] += x[p].z;
+            v[j + 3] += x[p].w;
           }
+        }
         lin_store<TO, NV>(a, (long long)m0 + r, n0 + c, v, b);
       }
     }
@@ -463,26 +499,37 @@ __global__ void __launch_bounds__(LN_THREADS, 1) lin_pair_kernel(const __grid_co
 }
 
 // LayerNorm of the rows (nn.cpp:73-83: biased variance, (x - mean) / sqrt(var
-// + eps) gamma + beta) into the GEMM's operand, rounded to its type: one CTA
-// per row, VPT vectors of 8 elements a thread in registers, two passes over
-// them in fp32.
+// + eps) gamma + beta) into the GEMM's operand, rounded to its type: two passes
+// over a row in fp32 registers, VPT vectors of 8 elements a thread. LANES 32: a
+// warp per row, four rows a CTA (rows of up to 2048); 128: a CTA per row.
 constexpr int LNORM_NT = 128;
-template <typename T, int VPT>
-__global__ void __launch_bounds__(LNORM_NT) lin_norm_kernel(const T* __restrict__ x, long long ldx, int K, bool vec,
-                                                            const float* __restrict__ gamma,
+template <typename T, int VPT, int LANES>
+__global__ void __launch_bounds__(LNORM_NT) lin_norm_kernel(const T* __restrict__ x, long long ldx, int M, int K,
+                                                            bool vec, const float* __restrict__ gamma,
                                                             const float* __restrict__ beta, float eps,
                                                             T* __restrict__ y) {
   __shared__ float red[2][LNORM_NT / 32];
   grid_dep_wait();
   grid_dep_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T* xr = x + (long long)blockIdx.x * ldx;
-  T* yr = y + (long long)blockIdx.x * K;
+  const int lane = threadIdx.x % LANES, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * (LNORM_NT / LANES) + threadIdx.x / LANES;
+  if (row >= M) return;                            // whole warps; LANES 128: whole CTAs
+  const T* xr = x + (long long)row * ldx;
+  T* yr = y + (long long)row * K;
+  auto sum = [&](float v, int which) {
+    v = warp_reduce(v, [](float a, float b) { return a + b; });
+    if constexpr (LANES > 32) {
+      if ((threadIdx.x & 31) == 0) red[which][warp] = v;
+      __syncthreads();
+      v = (red[which][0] + red[which][1]) + (red[which][2] + red[which][3]);
+    }
+    return v;
+  };
   float f[VPT][8];
   float s = 0.0f;
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const int k = (v * LNORM_NT + threadIdx.x) * 8;
+    const int k = (v * LANES + lane) * 8;
     T t[8];
     if (k < K) load8(xr + k, vec, t);
 #pragma unroll
@@ -491,35 +538,178 @@ __global__ void __launch_bounds__(LNORM_NT) lin_norm_kernel(const T* __restrict_
       s += f[v][i];
     }
   }
-  s = warp_reduce(s, [](float a, float b) { return a + b; });
-  if (lane == 0) red[0][warp] = s;
-  __syncthreads();
-  const float mean = ((red[0][0] + red[0][1]) + (red[0][2] + red[0][3])) / (float)K;
+  const float mean = sum(s, 0) / (float)K;
   float q = 0.0f;
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const bool in = (v * LNORM_NT + threadIdx.x) * 8 < K;
+    const bool in = (v * LANES + lane) * 8 < K;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       f[v][i] -= mean;
       q = in ? fmaf(f[v][i], f[v][i], q) : q;
     }
   }
-  q = warp_reduce(q, [](float a, float b) { return a + b; });
-  if (lane == 0) red[1][warp] = q;
-  __syncthreads();
-  const float rs = 1.0f / sqrtf(((red[1][0] + red[1][1]) + (red[1][2] + red[1][3])) / (float)K + eps);
+  const float rs = 1.0f / sqrtf(sum(q, 1) / (float)K + eps);
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const int k = (v * LNORM_NT + threadIdx.x) * 8;
+    const int k = (v * LANES + lane) * 8;
     if (k >= K) break;
+    float ga[8], be[8];
+    lin_gamma(gamma, beta, k, ga, be);
     T t[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      t[i] = Cvt<T>::t(fmaf(f[v][i] * rs, gamma ? __ldg(gamma + k + i) : 1.0f, beta ? __ldg(beta + k + i) : 0.0f));
+    for (int i = 0; i < 8; ++i) t[i] = Cvt<T>::t(fmaf(f[v][i] * rs, ga[i], be[i]));
     uint4 w;
     memcpy(&w, t, 16);
     *reinterpret_cast<uint4*>(yr + k) = w;
+  }
+}
+
+// ---- few rows: the weight streamed once through the warps --------------------
+// Decode steps of up to 8 MT streams read the whole weight for a few rows of x:
+// bound by HBM, and by latency at these sizes (13 MB take 2 us). One CTA takes
+// R rows of W, its eight warps interleaved 64-wide pieces of K: every 16-byte
+// load of W goes straight into the A fragments of mma.m16n8k16 (the order of K
+// inside a piece is the same for W and x, so no shuffle is needed), x's rows
+// are the eight columns. The warps' sums meet in shared memory. R is 8 (half of
+// the product's rows idle, twice the CTAs) where 16 would leave SMs without
+// work. The LayerNorm is done by every CTA for itself: a warp per row takes
+// mean and variance while the weight is on its way (prefetched to L2 before the
+// kernel waits for the one before it), and x is normalised, and rounded as the
+// other forms round it, as it is loaded.
+constexpr int LF_WARPS = 8;
+
+template <typename T>
+__device__ __forceinline__ void frag_mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                         unsigned b1) {
+  const unsigned a[4] = {a0, a1, a2, a3};
+  mma16816<T>(d, a, b0, b1);
+}
+
+template <typename TI, typename TO, int R, int MT>
+__global__ void __launch_bounds__(32 * LF_WARPS) lin_few_kernel(const TI* __restrict__ x, long long ldx, bool xvec,
+                                                                const float* __restrict__ gamma,
+                                                                const float* __restrict__ beta, float eps, bool norm,
+                                                                const TI* __restrict__ wt, long long ldw, LinArgs a) {
+  __shared__ float red[LF_WARPS][8 * MT][R + 1];
+  __shared__ float stat[8 * MT][2];                // mean, 1 / deviation
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * R;
+  {
+    // the weight's lines towards L2: no value is read before the wait
+    const int lines = (a.K * 2 + 127) / 128;
+    for (int i = threadIdx.x; i < R * lines; i += 32 * LF_WARPS) {
+      const int r = i / lines;
+      if (n0 + r < a.N) {
+        const char* p = reinterpret_cast<const char*>(wt + (long long)(n0 + r) * ldw) + (i - r * lines) * 128;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+      }
+    }
+  }
+  grid_dep_wait();
+  grid_dep_launch();
+  if (norm) {
+    for (int r = warp; r < a.M; r += LF_WARPS) {
+      const TI* xr = x + (long long)r * ldx;
+      float s = 0.0f, q = 0.0f;
+      for (int k = lane * 8; k < a.K; k += 256) {
+        TI v[8];
+        load8c(xr + k, xvec, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += Cvt<TI>::f(v[i]);
+      }
+      const float mean = warp_reduce(s, [](float p, float o) { return p + o; }) / (float)a.K;
+      for (int k = lane * 8; k < a.K; k += 256) {
+        TI v[8];
+        load8c(xr + k, xvec, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float d = Cvt<TI>::f(v[i]) - mean;
+          q = fmaf(d, d, q);
+        }
+      }
+      q = warp_reduce(q, [](float p, float o) { return p + o; });
+      if (lane == 0) {
+        stat[r][0] = mean;
+        stat[r][1] = 1.0f / sqrtf(q / (float)a.K + eps);
+      }
+    }
+    __syncthreads();
+  }
+  float acc[MT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[m][e] = 0.0f;
+  float mean[MT], rs[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const bool have = norm && m * 8 + g < a.M;
+    mean[m] = have ? stat[m * 8 + g][0] : 0.0f;
+    rs[m] = have ? stat[m * 8 + g][1] : 1.0f;
+  }
+  constexpr int UN = R == 16 ? 2 : 4;              // pieces in flight: eight 16-byte loads a lane
+  constexpr int RH = R / 8;
+  const TI* w0 = wt + (long long)min(n0 + g, a.N - 1) * ldw;           // a row past N repeats the last one, unused
+  const TI* w1 = wt + (long long)min(n0 + g + 8, a.N - 1) * ldw;
+  for (int k0 = warp * 64; k0 < a.K; k0 += UN * LF_WARPS * 64) {
+    uint4 wv[UN][2][RH];
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = k0 + u * LF_WARPS * 64 + h * 32 + t * 8;
+        const bool in = k < a.K;
+        wv[u][h][0] = in ? __ldcs(reinterpret_cast<const uint4*>(w0 + k)) : make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (RH == 2) wv[u][h][1] = in ? __ldcs(reinterpret_cast<const uint4*>(w1 + k)) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = k0 + u * LF_WARPS * 64 + h * 32 + t * 8;
+        uint4 xv[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          xv[m] = make_uint4(0u, 0u, 0u, 0u);
+          const int r = m * 8 + g;
+          if (k < a.K && r < a.M) {
+            TI v[8];
+            load8c(x + (long long)r * ldx + k, xvec, v);
+            if (norm) {
+              float ga[8], be[8];
+              lin_gamma(gamma, beta, k, ga, be);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = Cvt<TI>::t(fmaf((Cvt<TI>::f(v[i]) - mean[m]) * rs[m], ga[i], be[i]));
+            }
+            memcpy(&xv[m], v, 16);
+          }
+        }
+        const uint4 p = wv[u][h][0];
+        const uint4 q = RH == 2 ? wv[u][h][RH - 1] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          frag_mma<TI>(acc[m], p.x, q.x, p.y, q.y, xv[m].x, xv[m].y);
+          frag_mma<TI>(acc[m], p.z, q.z, p.w, q.w, xv[m].z, xv[m].w);
+        }
+      }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < 2 || R == 16) red[warp][m * 8 + 2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[m][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * a.M; i += 32 * LF_WARPS) {
+    const int m = i / R, r = i % R, n = n0 + r;
+    if (n >= a.N) continue;
+    float v[1] = {0.0f};
+#pragma unroll
+    for (int w = 0; w < LF_WARPS; ++w) v[0] += red[w][m][r];
+    if (a.bias) v[0] += __ldg(a.bias + n);
+    activate(v, a.act);
+    if (a.residual) v[0] += Cvt<TO>::f(static_cast<const TO*>(a.residual)[(long long)m * a.ldr + n]);
+    static_cast<TO*>(a.out)[(long long)m * a.ldo + n] = Cvt<TO>::t(v[0]);
   }
 }
 
