@@ -145,32 +145,66 @@ template <typename T, int NQ> AttnPick attn_pick_dim(int dim, int bits, int grou
                    : dim == 96 ? attn_pick_rows<T, 96, NQ>(bits, group) : attn_pick_rows<T, 128, NQ>(bits, group);
 }
 
-// 2-D tensor map of `outer` rows of `inner` 16-bit elements read in boxes of
-// 64 x `box` with the 128-byte swizzle; what lies outside reads as zeros.
+// 2-D tensor map of `outer` rows of `inner` elements in boxes of 128 bytes x
+// `box` rows with the 128-byte swizzle; what lies outside reads as zeros and
+// is not written.
 bool encode_rows(CUtensorMap* m, int dtype, const void* base, long long inner, long long outer, long long pitch_bytes,
                  int box) {
   const PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
   if (!enc) return false;
   cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
   cuuint64_t strides[1] = {(cuuint64_t)pitch_bytes};
-  cuuint32_t bx[2] = {(cuuint32_t)c4s::LN_BK, (cuuint32_t)box};
+  cuuint32_t bx[2] = {dtype == C4S_FP32 ? 32u : 64u, (cuuint32_t)box};
   cuuint32_t es[2] = {1, 1};
-  return enc(m, dtype == C4S_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+  return enc(m, dtype == C4S_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                : dtype == C4S_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
              const_cast<void*>(base), dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-using TileKernel = void (*)(const CUtensorMap, const CUtensorMap, c4s::LinArgs, int);
+using TileKernel = void (*)(const CUtensorMap, const CUtensorMap, c4s::LinArgs, int, int);
+using PairKernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, c4s::LinArgs);
 struct TilePick {
   TileKernel kern;
   size_t smem;
+  int stages;
 };
-// bn 64, 128: one CTA a tile; 256: pairs of CTAs
-template <typename TI, typename TO> TilePick tile_pick(int bn) {
-  if (bn == 256) return TilePick{c4s::lin_pair_kernel<TI, TO>, c4s::LP_SMEM};
-  return bn == 64 ? TilePick{c4s::lin_tile_kernel<TI, TO, 64>, c4s::LinCfg<64>::SMEM}
-                  : TilePick{c4s::lin_tile_kernel<TI, TO, 128>, c4s::LinCfg<128>::SMEM};
+// one CTA a tile, a ring of up to `room` bytes for x boxes of xbytes
+template <typename TI, typename TO> TilePick tile_pick(int bn, unsigned xbytes, size_t room) {
+  TilePick p;
+  if (bn == 64) {
+    p.kern = c4s::lin_tile_kernel<TI, TO, 64>;
+    c4s::LinCfg<64>::ring(xbytes, room, p.stages, p.smem);
+  } else {
+    p.kern = c4s::lin_tile_kernel<TI, TO, 128>;
+    c4s::LinCfg<128>::ring(xbytes, room, p.stages, p.smem);
+  }
+  return p;
 }
+
+// Launch in clusters of `cluster` CTAs along x.
+template <typename... P, typename... A>
+cudaError_t launch_cluster(void (*kern)(P...), dim3 grid, int cluster, int block, size_t smem, void* stream, A&&... args) {
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...);
+}
+
+bool aligned(const void* p, const void* q) { return (((uintptr_t)p | (uintptr_t)q) & 15) == 0; }
 
 template <typename T>
 cudaError_t launch_norm(const void* x, int M, int K, int64_t ldx, const float* gamma, const float* beta, float eps,
@@ -183,20 +217,20 @@ cudaError_t launch_norm(const void* x, int M, int K, int64_t ldx, const float* g
               : vpt <= 2 ? c4s::lin_norm_kernel<T, 2, 32>
               : vpt <= 5 ? c4s::lin_norm_kernel<T, 5, 32> : c4s::lin_norm_kernel<T, 8, 32>;
   return launch(kern, dim3((unsigned)((M + rows - 1) / rows)), c4s::LNORM_NT, 0, stream, (const T*)x, (long long)ldx, M,
-                K, vec, gamma, beta, eps, (T*)y);
+                K, vec, gamma, beta, aligned(gamma, beta), eps, (T*)y);
 }
 
-// The kernel for few rows (M <= 16).
+// The kernel for few rows. Sixteen warps a CTA where K is long.
 template <typename TI, typename TO>
 cudaError_t launch_few(const c4s_ctx* ctx, const void* x, long long ldx, const float* gamma, const float* beta, float eps,
                        bool norm, const void* w, long long ldw, const c4s::LinArgs& a, void* stream) {
   const bool xvec = ((uintptr_t)x & 15) == 0 && (ldx & 7) == 0;
-  const bool r16 = a.N >= 16 * ctx->num_sms;
-  auto kern = a.M <= 8 ? (r16 ? c4s::lin_few_kernel<TI, TO, 16, 1> : c4s::lin_few_kernel<TI, TO, 8, 1>)
-                       : (r16 ? c4s::lin_few_kernel<TI, TO, 16, 2> : c4s::lin_few_kernel<TI, TO, 8, 2>);
+  const bool r16 = a.N >= 16 * ctx->num_sms, w16 = false;
+  auto kern = r16 ? (w16 ? c4s::lin_few_kernel<TI, TO, 16, 16> : c4s::lin_few_kernel<TI, TO, 16, 8>)
+                  : (w16 ? c4s::lin_few_kernel<TI, TO, 8, 16> : c4s::lin_few_kernel<TI, TO, 8, 8>);
   const int R = r16 ? 16 : 8;
-  return launch(kern, dim3((unsigned)((a.N + R - 1) / R)), 32 * c4s::LF_WARPS, 0, stream, (const TI*)x, ldx, xvec, gamma,
-                beta, eps, norm, (const TI*)w, ldw, a);
+  return launch(kern, dim3((unsigned)((a.N + R - 1) / R)), w16 ? 512 : 256, 0, stream, (const TI*)x, ldx, xvec, gamma,
+                beta, aligned(gamma, beta), eps, norm, (const TI*)w, ldw, a);
 }
 
 // Workspace of the attention: for every warp of the grid two parts of up to 8
@@ -367,8 +401,9 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
   a.vec_out = ((uintptr_t)d_out & 15) == 0 && (ld_out * os) % 16 == 0;
   a.vec_res = ((uintptr_t)d_residual & 15) == 0 && (ld_residual * os) % 16 == 0;
   a.errflags = ctx->d_err;
+  a.vec_bias = ((uintptr_t)d_bias & 15) == 0;
   a.xbytes = 0;
-  if (M <= 16) {
+  if (M <= c4s::LF_ROWS) {
     const bool f32 = out_dtype == C4S_FP32, norm = d_norm != nullptr;
     e = dtype == C4S_BF16
             ? (f32 ? launch_few<__nv_bfloat16, float>(ctx, d_x, ld_x, d_gamma, d_beta, eps, norm, d_weight, ld_weight, a, stream)
@@ -384,42 +419,42 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
     d_x = d_norm;
     ld_x = K;
   }
-  // pairs of CTAs on 256 x 256 tiles where those fill the machine; else tiles of 128 columns where they do,
-  // else of 64, and clusters that share a tile's K
-  const int mt = (M + c4s::LN_BM - 1) / c4s::LN_BM, KB = (K + c4s::LN_BK - 1) / c4s::LN_BK;
+  const bool f32 = out_dtype == C4S_FP32;
   const long long big = (long long)((M + 255) / 256) * ((N + 255) / 256);
-  const bool pair = big * 2 >= ctx->num_sms;
-  const int bn = pair ? 256 : (long long)mt * ((N + 127) / 128) >= ctx->num_sms ? 128 : 64;
+  CUtensorMap tx, tw;
+  if (big * 2 >= ctx->num_sms) {
+    // pairs of CTAs on 256 x 256 tiles where those fill the machine
+    CUtensorMap to;
+    memset(&to, 0, sizeof(to));
+    if (!encode_rows(&tx, dtype, d_x, K, M, ld_x * 2, 128) || !encode_rows(&tw, dtype, d_weight, K, N, ld_weight * 2, 128) ||
+        (a.vec_out && !encode_rows(&to, out_dtype, d_out, N, M, ld_out * (long long)os, 32)))
+      return fail(ctx, C4S_ERR_CUDA, "tensor map encoding failed");
+    const PairKernel k = dtype == C4S_BF16
+                             ? (f32 ? c4s::lin_pair_kernel<__nv_bfloat16, float> : c4s::lin_pair_kernel<__nv_bfloat16, __nv_bfloat16>)
+                             : (f32 ? c4s::lin_pair_kernel<__half, float> : c4s::lin_pair_kernel<__half, __half>);
+    e = launch_cluster(k, dim3((unsigned)(2 * std::min<long long>(big, ctx->num_sms / 2))), 2, c4s::LP_THREADS,
+                       c4s::LP_SMEM, stream, tx, tw, to, a);
+    return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "linear launch");
+  }
+  // tiles of 128 columns where they fill the machine, else of 64, and clusters of 2, 4 or 8 CTAs that share a
+  // tile's K (other sizes leave SMs of a GPC without a cluster)
+  const int mt = (M + c4s::LN_BM - 1) / c4s::LN_BM, KB = (K + c4s::LN_BK - 1) / c4s::LN_BK;
+  const int bn = (long long)mt * ((N + 127) / 128) >= ctx->num_sms ? 128 : 64;
   const long long nt = (N + bn - 1) / bn;
   int S = 1;
-  while (!pair && S < 8 && nt * mt * S * 2 <= ctx->num_sms + ctx->num_sms / 4 && KB >= S * 2 * 4) S *= 2;
-  const int box = pair ? c4s::LN_BM : std::min(c4s::LN_BM, (M + 7) / 8 * 8);
-  CUtensorMap tx, tw;
-  if (!encode_rows(&tx, dtype, d_x, K, M, ld_x * 2, box) ||
-      !encode_rows(&tw, dtype, d_weight, K, N, ld_weight * 2, pair ? 128 : bn))
-    return fail(ctx, C4S_ERR_CUDA, "tensor map encoding failed");
+  while (S < c4s::LN_MAX_SPLIT && nt * mt * S * 2 <= ctx->num_sms + ctx->num_sms / 4 && KB >= S * 2 * 4) S *= 2;
+  const int box = std::min(c4s::LN_BM, (M + 7) / 8 * 8);
   a.xbytes = (unsigned)box * c4s::LN_BK * 2;
-  const TilePick k = dtype == C4S_BF16
-                         ? (out_dtype == C4S_FP32 ? tile_pick<__nv_bfloat16, float>(bn) : tile_pick<__nv_bfloat16, __nv_bfloat16>(bn))
-                         : (out_dtype == C4S_FP32 ? tile_pick<__half, float>(bn) : tile_pick<__half, __half>(bn));
-  e = cudaFuncSetAttribute(k.kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem);
-  if (e != cudaSuccess) return cuda_fail(ctx, e, "linear kernel attribute");
-  cudaLaunchConfig_t cfg = {};
-  const int cluster = pair ? 2 : S;
-  cfg.gridDim = pair ? dim3((unsigned)(2 * std::min<long long>(big, ctx->num_sms / 2))) : dim3((unsigned)(nt * S), (unsigned)mt);
-  cfg.blockDim = dim3(c4s::LN_THREADS);
-  cfg.dynamicSmemBytes = k.smem;
-  cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = (unsigned)cluster;
-  at[1].val.clusterDim.y = 1;
-  at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, k.kern, tx, tw, a, S);
+  // a whole SM's shared memory for a CTA where there are no more CTAs than SMs, else half of it
+  const size_t room = bn == 128 || nt * mt * S <= ctx->num_sms ? 225 * 1024 : 112 * 1024;
+  if (!encode_rows(&tx, dtype, d_x, K, M, ld_x * 2, box) || !encode_rows(&tw, dtype, d_weight, K, N, ld_weight * 2, bn))
+    return fail(ctx, C4S_ERR_CUDA, "tensor map encoding failed");
+  const TilePick k = dtype == C4S_BF16 ? (f32 ? tile_pick<__nv_bfloat16, float>(bn, a.xbytes, room)
+                                              : tile_pick<__nv_bfloat16, __nv_bfloat16>(bn, a.xbytes, room))
+                                       : (f32 ? tile_pick<__half, float>(bn, a.xbytes, room)
+                                              : tile_pick<__half, __half>(bn, a.xbytes, room));
+  e = launch_cluster(k.kern, dim3((unsigned)(nt * S), (unsigned)mt), S, c4s::LN_THREADS, k.smem, stream, tx, tw, a, S,
+                     k.stages);
   return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "linear launch");
 } catch (...) {
   return C4S_ERR_INVALID;

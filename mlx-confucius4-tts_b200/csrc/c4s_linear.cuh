@@ -25,8 +25,6 @@ constexpr int LN_BM = 128, LN_BK = 64;
 constexpr int LN_EPI_WARPS = 8;
 constexpr int LN_MAX_SPLIT = 8;                    // CTAs that share a tile's K
 constexpr int LN_THREADS = 64 + 32 * LN_EPI_WARPS;
-constexpr int LN_STAGE_PITCH = 36;                 // floats per row of a warp's 32 x 32 staging block (16-byte rows,
-                                                   // eight rows on different banks)
 
 // 8 consecutive elements of a row that several CTAs read.
 template <typename T>
@@ -39,12 +37,24 @@ __device__ __forceinline__ void load8c(const T* p, bool vec, T (&x)[8]) {
     for (int i = 0; i < 8; ++i) x[i] = p[i];
   }
 }
-// The norm's scale and shift of 8 consecutive columns (k a multiple of 8).
-__device__ __forceinline__ void lin_gamma(const float* gamma, const float* beta, int k, float (&ga)[8], float (&be)[8]) {
+// The norm's scale and shift of 8 consecutive columns (k a multiple of 8);
+// `vec`: both start on 16 bytes.
+__device__ __forceinline__ void lin_gamma(const float* gamma, const float* beta, bool vec, int k, float (&ga)[8],
+                                          float (&be)[8]) {
+  if (vec) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    ga[i] = gamma ? __ldg(gamma + k + i) : 1.0f;
-    be[i] = beta ? __ldg(beta + k + i) : 0.0f;
+    for (int i = 0; i < 8; i += 4) {
+      const float4 p = gamma ? __ldg(reinterpret_cast<const float4*>(gamma + k + i)) : make_float4(1.f, 1.f, 1.f, 1.f);
+      const float4 q = beta ? __ldg(reinterpret_cast<const float4*>(beta + k + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      ga[i] = p.x, ga[i + 1] = p.y, ga[i + 2] = p.z, ga[i + 3] = p.w;
+      be[i] = q.x, be[i + 1] = q.y, be[i + 2] = q.z, be[i + 3] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ga[i] = gamma ? __ldg(gamma + k + i) : 1.0f;
+      be[i] = beta ? __ldg(beta + k + i) : 0.0f;
+    }
   }
 }
 
@@ -56,7 +66,7 @@ struct LinArgs {
   long long ldo;
   int M, N, K;
   int act;                                         // C4S_ACT_*
-  bool vec_out, vec_res;                           // 16-byte aligned rows
+  bool vec_out, vec_res, vec_bias;                 // 16-byte aligned rows (from columns that are multiples of 32)
   unsigned xbytes;                                 // bytes of one TMA box of x
   unsigned* errflags;
 };
@@ -83,40 +93,55 @@ __device__ __forceinline__ void activate(float (&x)[N], int act) {
   }
 }
 
-// NV consecutive columns of bias from column n (zeros past N).
-template <int NV>
-__device__ __forceinline__ void lin_bias(const LinArgs& a, int n, float (&b)[NV]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i) b[i] = a.bias && n + i < a.N ? __ldg(a.bias + n + i) : 0.0f;
-}
-
-// NV consecutive outputs of a row from column n, given their sums of products:
-// bias, activation, residual, rounding, store.
+// NV consecutive outputs of a row from column n (n + i < N for those that
+// exist), given their sums of products: bias, activation, residual, one
+// rounding, 16-byte stores where the row allows them. The residual may be the
+// output itself: a thread reads what it then writes, before it writes.
 template <typename TO, int NV>
-__device__ __forceinline__ void lin_store(const LinArgs& a, long long row, int n, float (&v)[NV], const float (&b)[NV]) {
-  static_assert(NV * sizeof(TO) == 16, "one 16-byte store");
-  TO* o = static_cast<TO*>(a.out) + row * a.ldo + n;
+__device__ __forceinline__ void lin_finish(const LinArgs& a, long long row, int n, float (&v)[NV], TO (&x)[NV]) {
+  constexpr int PER = 16 / sizeof(TO);             // elements of one 16-byte piece
+  static_assert(NV % PER == 0 && NV % 4 == 0, "whole pieces");
   const bool full = n + NV <= a.N;
-  __align__(16) TO x[NV];
   if (a.residual) {
     const TO* r = static_cast<const TO*>(a.residual) + row * a.ldr + n;
     if (full && a.vec_res) {
-      *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(r);
+#pragma unroll
+      for (int i = 0; i < NV; i += PER) *reinterpret_cast<uint4*>(x + i) = *reinterpret_cast<const uint4*>(r + i);
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i) x[i] = n + i < a.N ? r[i] : Cvt<TO>::t(0.0f);
     }
   }
+  if (a.bias) {
+    const float* b = a.bias + n;
+    if (full && a.vec_bias) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) v[i] += b[i];
+      for (int i = 0; i < NV; i += 4) {
+        const float4 w = __ldg(reinterpret_cast<const float4*>(b + i));
+        v[i] += w.x, v[i + 1] += w.y, v[i + 2] += w.z, v[i + 3] += w.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (n + i < a.N) v[i] += __ldg(b + i);
+    }
+  }
   activate(v, a.act);
   if (a.residual)
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] += Cvt<TO>::f(x[i]);
 #pragma unroll
   for (int i = 0; i < NV; ++i) x[i] = Cvt<TO>::t(v[i]);
-  if (full && a.vec_out) {
-    *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(x);
+}
+template <typename TO, int NV>
+__device__ __forceinline__ void lin_store(const LinArgs& a, long long row, int n, float (&v)[NV]) {
+  constexpr int PER = 16 / sizeof(TO);
+  __align__(16) TO x[NV];
+  lin_finish(a, row, n, v, x);
+  TO* o = static_cast<TO*>(a.out) + row * a.ldo + n;
+  if (n + NV <= a.N && a.vec_out) {
+#pragma unroll
+    for (int i = 0; i < NV; i += PER) *reinterpret_cast<uint4*>(o + i) = *reinterpret_cast<const uint4*>(x + i);
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -124,42 +149,11 @@ __device__ __forceinline__ void lin_store(const LinArgs& a, long long row, int n
   }
 }
 
-// A warp's 32 x 32 block of the accumulator (TMEM lanes of its quarter, from
-// column tcol) to the output at row m0, column n0: lane = row on the way out of
-// TMEM, through the warp's staging block, then whole 16-byte pieces of rows.
-template <typename TO>
-__device__ __forceinline__ void lin_block(const LinArgs& a, unsigned taddr, float* st, long long m0, int n0, int lane) {
-  constexpr int NV = 16 / sizeof(TO), LPR = 32 / NV, RPI = 32 / LPR;   // lanes per row, rows per pass
-  const int c = (lane % LPR) * NV;
-  float b[NV];
-  lin_bias(a, n0 + c, b);
-  {
-    unsigned r[32];
-    tmem_ld32(taddr, r);
-    tmem_ld_wait();
-#pragma unroll
-    for (int j = 0; j < 32; j += 4)
-      *reinterpret_cast<float4*>(st + lane * LN_STAGE_PITCH + j) =
-          make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
-  }
-  __syncwarp();
-  if (n0 + c < a.N) {
-#pragma unroll 2
-    for (int i = 0; i < 32 / RPI; ++i) {
-      const int r = i * RPI + lane / LPR;
-      if (m0 + r >= a.M) break;
-      float v[NV];
-#pragma unroll
-      for (int j = 0; j < NV; j += 4)
-        *reinterpret_cast<float4*>(&v[j]) = *reinterpret_cast<const float4*>(st + r * LN_STAGE_PITCH + c + j);
-      lin_store<TO, NV>(a, m0 + r, n0 + c, v, b);
-    }
-  }
-  __syncwarp();
-}
-
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void umma_commit_at(unsigned bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ float4 ld_cluster(unsigned addr, unsigned rank) {
   unsigned p;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
@@ -176,31 +170,41 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, i
                : "memory");
 }
 
+// Ring of the tile kernel: stages of a W tile and the x rows that exist (a box
+// of up to 128), as many as fit. The product reads 128 rows of x whatever the
+// box: the rows behind it are whatever lies there (the slack at the ring's end
+// keeps that inside) and make accumulator rows that are never stored.
+constexpr int LT_MAX_ST = 12;
+
 template <int BN>
 struct LinCfg {
-  static constexpr unsigned XB = LN_BM * LN_BK * 2, WB = BN * LN_BK * 2;   // bytes of a stage's tiles
-  static constexpr int STAGES = BN <= 64 ? 4 : 6;                           // 64: two CTAs per SM
+  static constexpr unsigned WB = BN * LN_BK * 2;                           // bytes of a W tile
   static constexpr int PPITCH = BN + 4;                                    // floats per row of a split tile's partial
-  static constexpr size_t SMEM = STAGES * (size_t)(XB + WB) + 1024;
-  static_assert((size_t)LN_BM * PPITCH * 4 <= STAGES * (size_t)(XB + WB), "the partial fits the ring");
-  static_assert((size_t)LN_EPI_WARPS * 32 * LN_STAGE_PITCH * 4 <= STAGES * (size_t)(XB + WB), "and the staging blocks");
+  static constexpr size_t SLACK = LN_BM * LN_BK * 2;
+  static constexpr size_t FLOOR = (size_t)LN_BM * PPITCH * 4;              // a split tile's partial
+  // stages and bytes of shared memory for boxes of xbytes, `room` bytes at most
+  static void ring(unsigned xbytes, size_t room, int& st, size_t& smem) {
+    st = (int)((room - SLACK - 1024) / (WB + xbytes));
+    st = st < 2 ? 2 : st > LT_MAX_ST ? LT_MAX_ST : st;
+    smem = (size_t)st * (WB + xbytes) + SLACK;
+    smem = (smem > FLOOR ? smem : FLOOR) + 1024;
+  }
 };
 
 // TI: operands; TO: output; grid (ceil(N / BN) S, ceil(M / 128)), clusters of S along x.
 template <typename TI, typename TO, int BN>
 __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(const __grid_constant__ CUtensorMap tmX,
                                                                  const __grid_constant__ CUtensorMap tmW, LinArgs a,
-                                                                 int S) {
+                                                                 int S, int ST) {
   using Cfg = LinCfg<BN>;
-  constexpr int ST = Cfg::STAGES;
   constexpr unsigned BF = std::is_same<TI, __nv_bfloat16>::value ? 1u : 0u;
   constexpr unsigned IDESC = (1u << 4) | (BF << 7) | (BF << 10) | ((unsigned)(BN >> 3) << 17) | ((unsigned)(LN_BM >> 4) << 24);
   extern __shared__ unsigned char lsm_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<unsigned long long>(lsm_raw) + 1023ull) & ~1023ull);
-  __shared__ unsigned long long full[ST], empty[ST], accum;
+  __shared__ unsigned long long full[LT_MAX_ST], empty[LT_MAX_ST], accum;
   __shared__ unsigned tmem_base;
   __shared__ volatile int abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(FULL, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // known to be uniform
   const int s = (int)(blockIdx.x % (unsigned)S);
   const int n0 = (int)(blockIdx.x / (unsigned)S) * BN, m0 = blockIdx.y * LN_BM;
   const int KB = (a.K + LN_BK - 1) / LN_BK;
@@ -230,39 +234,52 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
     abort_flag = 1;
   };
   if (warp == 0) {
-    if (lane == 0) {
-      int it = 0;
-      for (; it < k1 - k0 && !abort_flag; ++it) {
-        const int i = it % ST;
-        if (!mbar_wait_1s(&empty[i], ((unsigned)(it / ST) & 1u) ^ 1u)) { give_up(); break; }
-        unsigned char* sx = ring + (size_t)i * (Cfg::XB + Cfg::WB);
-        mbar_arrive_expect_tx(&full[i], a.xbytes + Cfg::WB);
-        tma_load_2d(sx, &tmX, (k0 + it) * LN_BK, m0, &full[i]);
-        tma_load_2d(sx + Cfg::XB, &tmW, (k0 + it) * LN_BK, n0, &full[i]);
+    // whole warps walk the ring, one elected lane issues: what the issued instructions take stays in uniform registers
+    int it = 0, i = 0;
+    unsigned ph = 1, sw = smem_u32(ring);
+    const unsigned stage = Cfg::WB + a.xbytes, sw0 = sw, fb = smem_u32(full), eb = smem_u32(empty);
+    bool ok = true;
+    for (; it < k1 - k0; ++it) {
+      ok = mbar_wait_hot(eb + 8u * i, ph);
+      if (!ok) break;
+      if (elect_one()) {
+        mbar_expect_tx(fb + 8u * i, stage);
+        tma_tile(sw, &tmW, (k0 + it) * LN_BK, n0, fb + 8u * i);
+        tma_tile(sw + Cfg::WB, &tmX, (k0 + it) * LN_BK, m0, fb + 8u * i);
       }
-      // after a wait that gave up: the copies in flight land before the CTA goes
-      if (abort_flag)
-        for (int j = max(0, it - ST); j < it; ++j) mbar_wait_1s(&full[j % ST], (unsigned)(j / ST) & 1u);
+      __syncwarp();
+      sw += stage;
+      if (++i == ST) i = 0, ph ^= 1, sw = sw0;
     }
-    __syncwarp();
+    if (!ok) {
+      // a wait that gave up: the copies in flight land before the CTA goes
+      give_up();
+      for (int j = max(0, it - ST); j < it; ++j) mbar_wait_1s(&full[j % ST], (unsigned)(j / ST) & 1u);
+    }
   } else if (warp == 1) {
-    if (lane == 0) {
-      for (int it = 0; it < k1 - k0 && !abort_flag; ++it) {
-        const int i = it % ST;
-        if (!mbar_wait_1s(&full[i], (unsigned)(it / ST) & 1u)) { give_up(); break; }
-        tc_fence_after();
-        const unsigned char* sx = ring + (size_t)i * (Cfg::XB + Cfg::WB);
-        const unsigned long long xd = sw128_desc(sx), wd = sw128_desc(sx + Cfg::XB);
+    int i = 0;
+    unsigned ph = 0;
+    const unsigned fb = smem_u32(full), eb = smem_u32(empty);
+    const unsigned long long wd0 = sw128_desc(ring), step = (Cfg::WB + a.xbytes) >> 4;
+    unsigned long long wd = wd0;
+    for (int it = 0; it < k1 - k0; ++it) {
+      if (!mbar_wait_hot(fb + 8u * i, ph)) { give_up(); break; }
+      tc_fence_after();
+      if (elect_one()) {
+        const unsigned long long xd = wd + (Cfg::WB >> 4);
 #pragma unroll
         for (int kk = 0; kk < LN_BK / 16; ++kk)
           umma_f16(tmem, xd + 2ull * kk, wd + 2ull * kk, IDESC, (it | kk) != 0 ? 1u : 0u);
-        umma_commit(&empty[i]);
+        umma_commit_at(eb + 8u * i);
       }
-      umma_commit(&accum);
+      __syncwarp();
+      wd += step;
+      if (++i == ST) i = 0, ph ^= 1, wd = wd0;
     }
+    if (elect_one()) umma_commit(&accum);
     __syncwarp();
   } else {
-    const bool ok = mbar_wait_1s(&accum, 0u);
+    const bool ok = mbar_wait_warp(&accum, 0u);
     if (!ok) give_up();
     tc_fence_after();
     __syncwarp();
@@ -271,19 +288,17 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
     if (ok && !abort_flag && k1 > k0 && 32 * q < rows) {
       for (int c = half; c < BN / 32; c += 2) {
         const unsigned taddr = tmem + ((unsigned)(32 * q) << 16) + (unsigned)(32 * c);
+        float v[32];
+        tmem_ld32(taddr, reinterpret_cast<unsigned(&)[32]>(v));
+        tmem_ld_wait();
         if (S == 1) {
-          // staging blocks in the idle ring: every copy has landed and been read
-          lin_block<TO>(a, taddr, reinterpret_cast<float*>(ring) + (warp - 2) * 32 * LN_STAGE_PITCH,
-                        (long long)m0 + 32 * q, n0 + 32 * c, lane);
+          if (m0 + 32 * q + lane < a.M && n0 + 32 * c < a.N)
+            lin_store<TO, 32>(a, (long long)m0 + 32 * q + lane, n0 + 32 * c, v);
         } else {
-          unsigned r[32];
-          tmem_ld32(taddr, r);
-          tmem_ld_wait();
           float* p = reinterpret_cast<float*>(ring) + (32 * q + lane) * Cfg::PPITCH + 32 * c;
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<float4*>(p + j) = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
-                                                            __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+            *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         }
       }
     }
@@ -305,8 +320,7 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
       for (int i = threadIdx.x; i < (r1 - r0) * CG; i += LN_THREADS) {
         const int r = r0 + i / CG, c = (i % CG) * NV;
         if (n0 + c >= a.N) continue;
-        float v[NV], b[NV];
-        lin_bias(a, n0 + c, b);
+        float v[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) v[j] = 0.0f;
         const unsigned addr = smem_u32(ring) + (unsigned)(r * Cfg::PPITCH + c) * 4u;
@@ -324,7 +338,7 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
             v[j + 3] += x[p].w;
           }
         }
-        lin_store<TO, NV>(a, (long long)m0 + r, n0 + c, v, b);
+        lin_store<TO, NV>(a, (long long)m0 + r, n0 + c, v);
       }
     }
     cluster_arrive();
@@ -341,9 +355,15 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
 // columns), and the eight epilogue warps of each CTA finish a tile while the
 // next one's products run.
 constexpr int LP_ST = 5;                           // stages of the ring
+constexpr int LP_EPI_WARPS = 16;                   // four per TMEM lane quarter, 64 columns each
+constexpr int LP_THREADS = 64 + 32 * LP_EPI_WARPS;
 constexpr unsigned LP_HALF = 128 * LN_BK * 2;      // 16 KB: a CTA's rows of x, or of W, of one k-block
-constexpr size_t LP_STAGING = (size_t)LN_EPI_WARPS * 32 * LN_STAGE_PITCH * 4;
-constexpr size_t LP_SMEM = LP_ST * 2 * (size_t)LP_HALF + LP_STAGING + 1024;
+// A warp's block of the output on its way: 32 rows of 128 bytes (64 columns of
+// 16 bits, 32 of fp32), 16-byte pieces swizzled as the tensor map says. Written
+// by TMA, whole lines at once: 16-byte stores of one row a lane took 41 us of a
+// 49 us product (4099 x 1280 -> 5120).
+constexpr unsigned LP_OUT = 32 * 128;
+constexpr size_t LP_SMEM = LP_ST * 2 * (size_t)LP_HALF + LP_EPI_WARPS * (size_t)LP_OUT + 1024;
 
 __device__ __forceinline__ unsigned map_rank(unsigned addr, unsigned rank) {
   unsigned p;
@@ -351,10 +371,10 @@ __device__ __forceinline__ unsigned map_rank(unsigned addr, unsigned rank) {
   return p;
 }
 // A tile into this CTA's memory, counted on a barrier of the pair's first CTA.
-__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, unsigned bar) {
+__device__ __forceinline__ void tma_load_pair(unsigned dst, const CUtensorMap* map, int x, int y, unsigned bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
-      "[%4];" ::"r"(smem_u32(dst)),
+      "[%4];" ::"r"(dst),
       "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
@@ -377,18 +397,17 @@ __device__ __forceinline__ void umma_commit_pair(unsigned long long* bar) {
 }
 
 template <typename TI, typename TO>
-__global__ void __launch_bounds__(LN_THREADS, 1) lin_pair_kernel(const __grid_constant__ CUtensorMap tmX,
-                                                                 const __grid_constant__ CUtensorMap tmW, LinArgs a,
-                                                                 int) {
+__global__ void __launch_bounds__(LP_THREADS, 1) lin_pair_kernel(const __grid_constant__ CUtensorMap tmX,
+                                                                 const __grid_constant__ CUtensorMap tmW,
+                                                                 const __grid_constant__ CUtensorMap tmO, LinArgs a) {
   constexpr unsigned BF = std::is_same<TI, __nv_bfloat16>::value ? 1u : 0u;
   constexpr unsigned IDESC = (1u << 4) | (BF << 7) | (BF << 10) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
   extern __shared__ unsigned char lsm_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<unsigned long long>(lsm_raw) + 1023ull) & ~1023ull);
-  float* staging = reinterpret_cast<float*>(ring + LP_ST * 2 * (size_t)LP_HALF);
   __shared__ unsigned long long full[LP_ST], empty[LP_ST], acc_full[2], acc_empty[2];
   __shared__ unsigned tmem_base;
   __shared__ volatile int abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(FULL, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // known to be uniform
   const unsigned rank = blockIdx.x & 1u;           // in the pair
   const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
   const int KB = (a.K + LN_BK - 1) / LN_BK;
@@ -401,7 +420,7 @@ __global__ void __launch_bounds__(LN_THREADS, 1) lin_pair_kernel(const __grid_co
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 2 * LN_EPI_WARPS);  // both CTAs' epilogue warps
+      mbar_init(&acc_empty[i], 2 * LP_EPI_WARPS);  // both CTAs' epilogue warps
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -424,70 +443,125 @@ __global__ void __launch_bounds__(LN_THREADS, 1) lin_pair_kernel(const __grid_co
     abort_flag = 1;
   };
   if (warp == 0) {
-    if (lane == 0) {
-      // both CTAs copy their halves; the first CTA's barrier counts the bytes of both
-      int it = 0;
-      for (long long t = pair; t < tiles && !abort_flag; t += pairs) {
-        const int m0 = (int)(t % mt) * 256 + (int)rank * 128, n0 = (int)(t / mt) * 256 + (int)rank * 128;
-        for (int kb = 0; kb < KB && !abort_flag; ++kb, ++it) {
-          const int i = it % LP_ST;
-          if (!mbar_wait_1s(&empty[i], ((unsigned)(it / LP_ST) & 1u) ^ 1u)) { give_up(); break; }
-          unsigned char* sx = ring + (size_t)i * 2 * LP_HALF;
-          const unsigned bar = map_rank(smem_u32(&full[i]), 0u);
-          if (rank == 0) mbar_arrive_expect_tx(&full[i], 4 * LP_HALF);
+    // both CTAs copy their halves; the first CTA's barrier counts the bytes of both
+    int it = 0, i = 0;
+    unsigned ph = 1;
+    const unsigned s0 = smem_u32(ring), fb = smem_u32(full), eb = smem_u32(empty), lead = map_rank(fb, 0u);
+    bool ok = true;
+    for (long long t = pair; ok && t < tiles; t += pairs) {
+      const int m0 = (int)(t % mt) * 256 + (int)rank * 128, n0 = (int)(t / mt) * 256 + (int)rank * 128;
+      for (int kb = 0; kb < KB; ++kb, ++it) {
+        ok = mbar_wait_hot(eb + 8u * i, ph);
+        if (!ok) break;
+        if (elect_one()) {
+          const unsigned sx = s0 + (unsigned)i * 2 * LP_HALF, bar = lead + 8u * i;
+          if (rank == 0) mbar_expect_tx(fb + 8u * i, 4 * LP_HALF);
           tma_load_pair(sx, &tmX, kb * LN_BK, m0, bar);
           tma_load_pair(sx + LP_HALF, &tmW, kb * LN_BK, n0, bar);
         }
+        __syncwarp();
+        if (++i == LP_ST) i = 0, ph ^= 1;
       }
-      // after a wait that gave up: the copies in flight land before the pair goes
-      if (abort_flag && rank == 0)
+    }
+    if (!ok) {
+      // a wait that gave up: the copies in flight land before the pair goes
+      give_up();
+      if (rank == 0)
         for (int j = max(0, it - LP_ST); j < it; ++j) mbar_wait_1s(&full[j % LP_ST], (unsigned)(j / LP_ST) & 1u);
     }
-    __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      int it = 0, n = 0;
-      for (long long t = pair; t < tiles && !abort_flag; t += pairs, ++n) {
+    if (rank == 0) {
+      int n = 0, i = 0;
+      unsigned ph = 0;
+      const unsigned fb = smem_u32(full), ab = smem_u32(acc_empty);
+      const unsigned long long d0 = sw128_desc(ring);
+      bool ok = true;
+      for (long long t = pair; ok && t < tiles; t += pairs, ++n) {
         const int buf = n & 1;
-        if (!mbar_wait_1s(&acc_empty[buf], ((unsigned)(n >> 1) & 1u) ^ 1u)) { give_up(); break; }
+        ok = mbar_wait_hot(ab + 8u * buf, ((unsigned)(n >> 1) & 1u) ^ 1u);
+        if (!ok) { give_up(); break; }
         tc_fence_after();
-        for (int kb = 0; kb < KB && !abort_flag; ++kb, ++it) {
-          const int i = it % LP_ST;
-          if (!mbar_wait_1s(&full[i], (unsigned)(it / LP_ST) & 1u)) { give_up(); break; }
+        for (int kb = 0; kb < KB; ++kb) {
+          ok = mbar_wait_hot(fb + 8u * i, ph);
+          if (!ok) { give_up(); break; }
           tc_fence_after();
-          const unsigned char* sx = ring + (size_t)i * 2 * LP_HALF;
-          const unsigned long long xd = sw128_desc(sx), wd = sw128_desc(sx + LP_HALF);
+          if (elect_one()) {
+            const unsigned long long xd = d0 + (unsigned)i * (2 * LP_HALF >> 4), wd = xd + (LP_HALF >> 4);
 #pragma unroll
-          for (int kk = 0; kk < LN_BK / 16; ++kk)
-            umma_pair(tmem + (unsigned)(buf * 256), xd + 2ull * kk, wd + 2ull * kk, IDESC, (kb | kk) != 0 ? 1u : 0u);
-          umma_commit_pair(&empty[i]);
+            for (int kk = 0; kk < LN_BK / 16; ++kk)
+              umma_pair(tmem + (unsigned)(buf * 256), xd + 2ull * kk, wd + 2ull * kk, IDESC, (kb | kk) != 0 ? 1u : 0u);
+            umma_commit_pair(&empty[i]);
+          }
+          __syncwarp();
+          if (++i == LP_ST) i = 0, ph ^= 1;
         }
-        umma_commit_pair(&acc_full[buf]);
+        if (elect_one()) umma_commit_pair(&acc_full[buf]);
+        __syncwarp();
       }
     }
-    __syncwarp();
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    float* st = staging + (warp - 2) * 32 * LN_STAGE_PITCH;
+    const int q = warp & 3, cg = (warp - 2) >> 2;              // TMEM lane quarter, 64-column group
+    const unsigned obuf = smem_u32(ring) + LP_ST * 2 * LP_HALF + (unsigned)(warp - 2) * LP_OUT;
     int n = 0;
     for (long long t = pair; t < tiles; t += pairs, ++n) {
       const int buf = n & 1;
       const long long m0 = (t % mt) * 256 + rank * 128 + 32 * q;
-      const int n0 = (int)(t / mt) * 256;
-      const bool ok = mbar_wait_1s(&acc_full[buf], (unsigned)(n >> 1) & 1u);
+      const int n0 = (int)(t / mt) * 256 + 64 * cg;
+      const bool ok = mbar_wait_warp(&acc_full[buf], (unsigned)(n >> 1) & 1u);
       if (!ok) give_up();
       tc_fence_after();
       if (!__all_sync(FULL, ok) || abort_flag) break;
-      if (m0 < a.M)
-        for (int c = 4 * half; c < 4 * half + 4 && n0 + 32 * c < a.N; ++c)
-          lin_block<TO>(a, tmem + ((unsigned)(32 * q) << 16) + (unsigned)(buf * 256 + 32 * c), st, m0, n0 + 32 * c, lane);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        const unsigned bar = map_rank(smem_u32(&acc_empty[buf]), 0u);
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+      const unsigned taddr = tmem + ((unsigned)(32 * q) << 16) + (unsigned)(buf * 256 + 64 * cg);
+      const bool tma = a.vec_out;                  // rows that a tensor map can name
+      constexpr int PER = 16 / sizeof(TO), PIECES = 32 / PER;  // 16-byte pieces of a row's 32 columns
+      constexpr bool ONE = PIECES == 4;            // both halves of the 64 columns make one block
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        float v[32];
+        tmem_ld32(taddr + 32u * c, reinterpret_cast<unsigned(&)[32]>(v));
+        tmem_ld_wait();
+        if (c == 1) {                              // out of TMEM: the buffer is free for the products after next
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            const unsigned bar = map_rank(smem_u32(&acc_empty[buf]), 0u);
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+          }
+        }
+        if (n0 + 32 * c >= a.N || m0 >= a.M) continue;         // uniform
+        if (!tma) {
+          if (m0 + lane < a.M) lin_store<TO, 32>(a, m0 + lane, n0 + 32 * c, v);
+          continue;
+        }
+        __align__(16) TO x[32];
+        // rows past M repeat the last one's residual; the tensor map cuts them
+        lin_finish(a, min(m0 + lane, (long long)a.M - 1), n0 + 32 * c, v, x);
+        if (c == 0 || !ONE) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the block before has been read
+          __syncwarp();
+        }
+        const unsigned row = obuf + lane * 128u;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const uint4 w = *reinterpret_cast<const uint4*>(x + i * PER);
+          const unsigned at = row + ((((ONE ? 4 * c : 0) + i) ^ (lane & 7)) << 4);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+        }
+        if (!ONE || c == 1 || n0 + 32 >= a.N) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                             reinterpret_cast<unsigned long long>(&tmO)),
+                         "r"(n0 + (ONE ? 0 : 32 * c)), "r"((int)m0), "r"(obuf)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        }
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the output is written
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -506,7 +580,7 @@ constexpr int LNORM_NT = 128;
 template <typename T, int VPT, int LANES>
 __global__ void __launch_bounds__(LNORM_NT) lin_norm_kernel(const T* __restrict__ x, long long ldx, int M, int K,
                                                             bool vec, const float* __restrict__ gamma,
-                                                            const float* __restrict__ beta, float eps,
+                                                            const float* __restrict__ beta, bool gvec, float eps,
                                                             T* __restrict__ y) {
   __shared__ float red[2][LNORM_NT / 32];
   grid_dep_wait();
@@ -555,7 +629,7 @@ __global__ void __launch_bounds__(LNORM_NT) lin_norm_kernel(const T* __restrict_
     const int k = (v * LANES + lane) * 8;
     if (k >= K) break;
     float ga[8], be[8];
-    lin_gamma(gamma, beta, k, ga, be);
+    lin_gamma(gamma, beta, gvec, k, ga, be);
     T t[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = Cvt<T>::t(fmaf(f[v][i] * rs, ga[i], be[i]));
@@ -566,9 +640,9 @@ __global__ void __launch_bounds__(LNORM_NT) lin_norm_kernel(const T* __restrict_
 }
 
 // ---- few rows: the weight streamed once through the warps --------------------
-// Decode steps of up to 8 MT streams read the whole weight for a few rows of x:
+// Decode steps of up to 8 streams read the whole weight for a few rows of x:
 // bound by HBM, and by latency at these sizes (13 MB take 2 us). One CTA takes
-// R rows of W, its eight warps interleaved 64-wide pieces of K: every 16-byte
+// R rows of W, its WARPS warps interleaved 64-wide pieces of K: every 16-byte
 // load of W goes straight into the A fragments of mma.m16n8k16 (the order of K
 // inside a piece is the same for W and x, so no shuffle is needed), x's rows
 // are the eight columns. The warps' sums meet in shared memory. R is 8 (half of
@@ -577,28 +651,22 @@ __global__ void __launch_bounds__(LNORM_NT) lin_norm_kernel(const T* __restrict_
 // mean and variance while the weight is on its way (prefetched to L2 before the
 // kernel waits for the one before it), and x is normalised, and rounded as the
 // other forms round it, as it is loaded.
-constexpr int LF_WARPS = 8;
+constexpr int LF_ROWS = 8;
 
-template <typename T>
-__device__ __forceinline__ void frag_mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
-                                         unsigned b1) {
-  const unsigned a[4] = {a0, a1, a2, a3};
-  mma16816<T>(d, a, b0, b1);
-}
-
-template <typename TI, typename TO, int R, int MT>
-__global__ void __launch_bounds__(32 * LF_WARPS) lin_few_kernel(const TI* __restrict__ x, long long ldx, bool xvec,
-                                                                const float* __restrict__ gamma,
-                                                                const float* __restrict__ beta, float eps, bool norm,
-                                                                const TI* __restrict__ wt, long long ldw, LinArgs a) {
-  __shared__ float red[LF_WARPS][8 * MT][R + 1];
-  __shared__ float stat[8 * MT][2];                // mean, 1 / deviation
+template <typename TI, typename TO, int R, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) lin_few_kernel(const TI* __restrict__ x, long long ldx, bool xvec,
+                                                             const float* __restrict__ gamma,
+                                                             const float* __restrict__ beta, bool gvec, float eps,
+                                                             bool norm, const TI* __restrict__ wt, long long ldw,
+                                                             LinArgs a) {
+  __shared__ float red[WARPS][LF_ROWS][R + 1];
+  __shared__ float stat[LF_ROWS][2];               // mean, 1 / deviation
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * R;
   {
     // the weight's lines towards L2: no value is read before the wait
     const int lines = (a.K * 2 + 127) / 128;
-    for (int i = threadIdx.x; i < R * lines; i += 32 * LF_WARPS) {
+    for (int i = threadIdx.x; i < R * lines; i += 32 * WARPS) {
       const int r = i / lines;
       if (n0 + r < a.N) {
         const char* p = reinterpret_cast<const char*>(wt + (long long)(n0 + r) * ldw) + (i - r * lines) * 128;
@@ -609,9 +677,10 @@ __global__ void __launch_bounds__(32 * LF_WARPS) lin_few_kernel(const TI* __rest
   grid_dep_wait();
   grid_dep_launch();
   if (norm) {
-    for (int r = warp; r < a.M; r += LF_WARPS) {
+    for (int r = warp; r < a.M; r += WARPS) {
       const TI* xr = x + (long long)r * ldx;
       float s = 0.0f, q = 0.0f;
+#pragma unroll 4
       for (int k = lane * 8; k < a.K; k += 256) {
         TI v[8];
         load8c(xr + k, xvec, v);
@@ -619,6 +688,7 @@ __global__ void __launch_bounds__(32 * LF_WARPS) lin_few_kernel(const TI* __rest
         for (int i = 0; i < 8; ++i) s += Cvt<TI>::f(v[i]);
       }
       const float mean = warp_reduce(s, [](float p, float o) { return p + o; }) / (float)a.K;
+#pragma unroll 4
       for (int k = lane * 8; k < a.K; k += 256) {
         TI v[8];
         load8c(xr + k, xvec, v);
@@ -636,29 +706,20 @@ __global__ void __launch_bounds__(32 * LF_WARPS) lin_few_kernel(const TI* __rest
     }
     __syncthreads();
   }
-  float acc[MT][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[m][e] = 0.0f;
-  float mean[MT], rs[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const bool have = norm && m * 8 + g < a.M;
-    mean[m] = have ? stat[m * 8 + g][0] : 0.0f;
-    rs[m] = have ? stat[m * 8 + g][1] : 1.0f;
-  }
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const bool mine = g < a.M;
+  const float mean = norm && mine ? stat[g][0] : 0.0f, rs = norm && mine ? stat[g][1] : 1.0f;
   constexpr int UN = R == 16 ? 2 : 4;              // pieces in flight: eight 16-byte loads a lane
   constexpr int RH = R / 8;
   const TI* w0 = wt + (long long)min(n0 + g, a.N - 1) * ldw;           // a row past N repeats the last one, unused
   const TI* w1 = wt + (long long)min(n0 + g + 8, a.N - 1) * ldw;
-  for (int k0 = warp * 64; k0 < a.K; k0 += UN * LF_WARPS * 64) {
+  for (int k0 = warp * 64; k0 < a.K; k0 += UN * WARPS * 64) {
     uint4 wv[UN][2][RH];
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = k0 + u * LF_WARPS * 64 + h * 32 + t * 8;
+        const int k = k0 + u * WARPS * 64 + h * 32 + t * 8;
         const bool in = k < a.K;
         wv[u][h][0] = in ? __ldcs(reinterpret_cast<const uint4*>(w0 + k)) : make_uint4(0u, 0u, 0u, 0u);
         if constexpr (RH == 2) wv[u][h][1] = in ? __ldcs(reinterpret_cast<const uint4*>(w1 + k)) : make_uint4(0u, 0u, 0u, 0u);
@@ -667,45 +728,35 @@ __global__ void __launch_bounds__(32 * LF_WARPS) lin_few_kernel(const TI* __rest
     for (int u = 0; u < UN; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = k0 + u * LF_WARPS * 64 + h * 32 + t * 8;
-        uint4 xv[MT];
+        const int k = k0 + u * WARPS * 64 + h * 32 + t * 8;
+        uint4 xv = make_uint4(0u, 0u, 0u, 0u);
+        if (k < a.K && mine) {
+          TI v[8];
+          load8c(x + (long long)g * ldx + k, xvec, v);
+          if (norm) {
+            float ga[8], be[8];
+            lin_gamma(gamma, beta, gvec, k, ga, be);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          xv[m] = make_uint4(0u, 0u, 0u, 0u);
-          const int r = m * 8 + g;
-          if (k < a.K && r < a.M) {
-            TI v[8];
-            load8c(x + (long long)r * ldx + k, xvec, v);
-            if (norm) {
-              float ga[8], be[8];
-              lin_gamma(gamma, beta, k, ga, be);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = Cvt<TI>::t(fmaf((Cvt<TI>::f(v[i]) - mean[m]) * rs[m], ga[i], be[i]));
-            }
-            memcpy(&xv[m], v, 16);
+            for (int i = 0; i < 8; ++i) v[i] = Cvt<TI>::t(fmaf((Cvt<TI>::f(v[i]) - mean) * rs, ga[i], be[i]));
           }
+          memcpy(&xv, v, 16);
         }
         const uint4 p = wv[u][h][0];
         const uint4 q = RH == 2 ? wv[u][h][RH - 1] : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          frag_mma<TI>(acc[m], p.x, q.x, p.y, q.y, xv[m].x, xv[m].y);
-          frag_mma<TI>(acc[m], p.z, q.z, p.w, q.w, xv[m].z, xv[m].w);
-        }
+        const unsigned a0[4] = {p.x, q.x, p.y, q.y}, a1[4] = {p.z, q.z, p.w, q.w};
+        mma16816<TI>(acc, a0, xv.x, xv.y);
+        mma16816<TI>(acc, a1, xv.z, xv.w);
       }
   }
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < 2 || R == 16) red[warp][m * 8 + 2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[m][e];
+  for (int e = 0; e < 2 * RH; ++e) red[warp][2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[e];
   __syncthreads();
-  for (int i = threadIdx.x; i < R * a.M; i += 32 * LF_WARPS) {
+  for (int i = threadIdx.x; i < R * a.M; i += 32 * WARPS) {
     const int m = i / R, r = i % R, n = n0 + r;
     if (n >= a.N) continue;
     float v[1] = {0.0f};
 #pragma unroll
-    for (int w = 0; w < LF_WARPS; ++w) v[0] += red[w][m][r];
+    for (int w = 0; w < WARPS; ++w) v[0] += red[w][m][r];
     if (a.bias) v[0] += __ldg(a.bias + n);
     activate(v, a.act);
     if (a.residual) v[0] += Cvt<TO>::f(static_cast<const TO*>(a.residual)[(long long)m * a.ldr + n]);

@@ -78,4 +78,81 @@ __device__ __forceinline__ bool mbar_wait_1s(unsigned long long* bar, unsigned p
   return false;
 }
 
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  unsigned p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// The same for a warp that feeds a pipeline, on a shared-memory address: a
+// tight loop first, the timer only after many tries.
+__device__ __forceinline__ bool mbar_wait_hot(unsigned bar, unsigned parity) {
+  unsigned ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, 0;\n"
+      "C4S_TRY:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra C4S_DONE;\n\t"
+      "add.u32 n, n, 1;\n\t"
+      "setp.lt.u32 p, n, 4096;\n\t"
+      "@p bra C4S_TRY;\n"
+      "C4S_DONE:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (ok) return true;
+  const unsigned long long t0 = globaltimer_ns();
+  for (unsigned it = 0; it < (1u << 30); ++it) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 63u) == 63u && globaltimer_ns() - t0 > 1000000000ull) return false;
+  }
+  return false;
+}
+__device__ __forceinline__ void mbar_expect_tx(unsigned bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_tile(unsigned dst, const CUtensorMap* map, int x, int y, unsigned bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
+          "r"(dst),
+      "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+// The same for a whole warp that has nothing else to do: one lane polls, with
+// pauses. Warps that all spin on a barrier take the issue slots and the
+// shared-memory path of the two lanes that feed the pipeline: with eight of
+// them spinning, a k-block took 640 cycles whatever its bytes.
+__device__ __forceinline__ bool mbar_wait_warp(unsigned long long* bar, unsigned parity) {
+  unsigned ok = 0;
+  if ((threadIdx.x & 31) == 0) {
+    ok = mbar_try_wait(bar, parity);
+    if (!ok) {
+      const unsigned long long t0 = globaltimer_ns();
+      for (unsigned it = 0; it < (1u << 28) && !ok; ++it) {
+        __nanosleep(64);
+        ok = mbar_try_wait(bar, parity);
+        if ((it & 63u) == 63u && globaltimer_ns() - t0 > 1000000000ull) break;
+      }
+    }
+  }
+  ok = __shfl_sync(FULL, ok, 0);
+  // every lane passes the barrier itself, for what it orders
+  return ok && mbar_wait_1s(bar, parity);
+}
+
 }  // namespace c4s
