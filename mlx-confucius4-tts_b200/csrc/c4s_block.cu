@@ -432,8 +432,8 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
     const PairKernel k = dtype == C4S_BF16
                              ? (f32 ? c4s::lin_pair_kernel<__nv_bfloat16, float> : c4s::lin_pair_kernel<__nv_bfloat16, __nv_bfloat16>)
                              : (f32 ? c4s::lin_pair_kernel<__half, float> : c4s::lin_pair_kernel<__half, __half>);
-    e = launch_cluster(k, dim3((unsigned)(2 * std::min<long long>(big, ctx->num_sms / 2))), 2, c4s::LP_THREADS,
-                       c4s::LP_SMEM, stream, tx, tw, to, a);
+    e = launch_cluster(k, dim3((unsigned)(2 * std::min<long long>(big, ctx->num_sms / 2))), 2, f32 ? c4s::LpCfg<float>::THREADS : c4s::LpCfg<__half>::THREADS,
+                       f32 ? c4s::LpCfg<float>::SMEM : c4s::LpCfg<__half>::SMEM, stream, tx, tw, to, a);
     return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "linear launch");
   }
   // tiles of 128 columns where they fill the machine, else of 64, and clusters of 2, 4 or 8 CTAs that share a

@@ -354,16 +354,21 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
 // take tiles in turn, the accumulator is double-buffered in TMEM (2 x 256
 // columns), and the eight epilogue warps of each CTA finish a tile while the
 // next one's products run.
-constexpr int LP_ST = 5;                           // stages of the ring
-constexpr int LP_EPI_WARPS = 16;                   // four per TMEM lane quarter, 64 columns each
-constexpr int LP_THREADS = 64 + 32 * LP_EPI_WARPS;
 constexpr unsigned LP_HALF = 128 * LN_BK * 2;      // 16 KB: a CTA's rows of x, or of W, of one k-block
 // A warp's block of the output on its way: 32 rows of 128 bytes (64 columns of
 // 16 bits, 32 of fp32), 16-byte pieces swizzled as the tensor map says. Written
 // by TMA, whole lines at once: 16-byte stores of one row a lane took 41 us of a
 // 49 us product (4099 x 1280 -> 5120).
 constexpr unsigned LP_OUT = 32 * 128;
-constexpr size_t LP_SMEM = LP_ST * 2 * (size_t)LP_HALF + LP_EPI_WARPS * (size_t)LP_OUT + 1024;
+// Sixteen epilogue warps hide the activation's latency best (GELU: 42.5 us
+// there, 45.2 with eight); fp32 outputs take more registers than those leave.
+template <typename TO>
+struct LpCfg {
+  static constexpr int EPI = sizeof(TO) == 2 ? 16 : 8;         // epilogue warps
+  static constexpr int ST = EPI == 16 ? 5 : 6;                 // stages of the ring
+  static constexpr int THREADS = 64 + 32 * EPI;
+  static constexpr size_t SMEM = ST * 2 * (size_t)LP_HALF + EPI * (size_t)LP_OUT + 1024;
+};
 
 __device__ __forceinline__ unsigned map_rank(unsigned addr, unsigned rank) {
   unsigned p;
@@ -397,14 +402,15 @@ __device__ __forceinline__ void umma_commit_pair(unsigned long long* bar) {
 }
 
 template <typename TI, typename TO>
-__global__ void __launch_bounds__(LP_THREADS, 1) lin_pair_kernel(const __grid_constant__ CUtensorMap tmX,
+__global__ void __launch_bounds__(LpCfg<TO>::THREADS, 1) lin_pair_kernel(const __grid_constant__ CUtensorMap tmX,
                                                                  const __grid_constant__ CUtensorMap tmW,
                                                                  const __grid_constant__ CUtensorMap tmO, LinArgs a) {
+  constexpr int ST = LpCfg<TO>::ST, EPI = LpCfg<TO>::EPI;
   constexpr unsigned BF = std::is_same<TI, __nv_bfloat16>::value ? 1u : 0u;
   constexpr unsigned IDESC = (1u << 4) | (BF << 7) | (BF << 10) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
   extern __shared__ unsigned char lsm_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<unsigned long long>(lsm_raw) + 1023ull) & ~1023ull);
-  __shared__ unsigned long long full[LP_ST], empty[LP_ST], acc_full[2], acc_empty[2];
+  __shared__ unsigned long long full[ST], empty[ST], acc_full[2], acc_empty[2];
   __shared__ unsigned tmem_base;
   __shared__ volatile int abort_flag;
   const int warp = __shfl_sync(FULL, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // known to be uniform
@@ -414,13 +420,13 @@ __global__ void __launch_bounds__(LP_THREADS, 1) lin_pair_kernel(const __grid_co
   const int mt = (a.M + 255) / 256, nt = (a.N + 255) / 256;
   const long long tiles = (long long)mt * nt;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < LP_ST; ++i) {
+    for (int i = 0; i < ST; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 2 * LP_EPI_WARPS);  // both CTAs' epilogue warps
+      mbar_init(&acc_empty[i], 2 * EPI);  // both CTAs' epilogue warps
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -460,14 +466,14 @@ __global__ void __launch_bounds__(LP_THREADS, 1) lin_pair_kernel(const __grid_co
           tma_load_pair(sx + LP_HALF, &tmW, kb * LN_BK, n0, bar);
         }
         __syncwarp();
-        if (++i == LP_ST) i = 0, ph ^= 1;
+        if (++i == ST) i = 0, ph ^= 1;
       }
     }
     if (!ok) {
       // a wait that gave up: the copies in flight land before the pair goes
       give_up();
       if (rank == 0)
-        for (int j = max(0, it - LP_ST); j < it; ++j) mbar_wait_1s(&full[j % LP_ST], (unsigned)(j / LP_ST) & 1u);
+        for (int j = max(0, it - ST); j < it; ++j) mbar_wait_1s(&full[j % ST], (unsigned)(j / ST) & 1u);
     }
   } else if (warp == 1) {
     if (rank == 0) {
@@ -493,34 +499,35 @@ __global__ void __launch_bounds__(LP_THREADS, 1) lin_pair_kernel(const __grid_co
             umma_commit_pair(&empty[i]);
           }
           __syncwarp();
-          if (++i == LP_ST) i = 0, ph ^= 1;
+          if (++i == ST) i = 0, ph ^= 1;
         }
         if (elect_one()) umma_commit_pair(&acc_full[buf]);
         __syncwarp();
       }
     }
   } else {
-    const int q = warp & 3, cg = (warp - 2) >> 2;              // TMEM lane quarter, 64-column group
-    const unsigned obuf = smem_u32(ring) + LP_ST * 2 * LP_HALF + (unsigned)(warp - 2) * LP_OUT;
+    constexpr int CW = 256 / (EPI / 4);               // columns of a warp
+    const int q = warp & 3, cg = (warp - 2) >> 2;              // TMEM lane quarter, column group
+    const unsigned obuf = smem_u32(ring) + ST * 2 * LP_HALF + (unsigned)(warp - 2) * LP_OUT;
     int n = 0;
     for (long long t = pair; t < tiles; t += pairs, ++n) {
       const int buf = n & 1;
       const long long m0 = (t % mt) * 256 + rank * 128 + 32 * q;
-      const int n0 = (int)(t / mt) * 256 + 64 * cg;
+      const int n0 = (int)(t / mt) * 256 + CW * cg;
       const bool ok = mbar_wait_warp(&acc_full[buf], (unsigned)(n >> 1) & 1u);
       if (!ok) give_up();
       tc_fence_after();
       if (!__all_sync(FULL, ok) || abort_flag) break;
-      const unsigned taddr = tmem + ((unsigned)(32 * q) << 16) + (unsigned)(buf * 256 + 64 * cg);
+      const unsigned taddr = tmem + ((unsigned)(32 * q) << 16) + (unsigned)(buf * 256 + CW * cg);
       const bool tma = a.vec_out;                  // rows that a tensor map can name
       constexpr int PER = 16 / sizeof(TO), PIECES = 32 / PER;  // 16-byte pieces of a row's 32 columns
       constexpr bool ONE = PIECES == 4;            // both halves of the 64 columns make one block
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < CW / 32; ++c) {
         float v[32];
         tmem_ld32(taddr + 32u * c, reinterpret_cast<unsigned(&)[32]>(v));
         tmem_ld_wait();
-        if (c == 1) {                              // out of TMEM: the buffer is free for the products after next
+        if (c == CW / 32 - 1) {                    // out of TMEM: the buffer is free for the products after next
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -536,7 +543,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1) lin_pair_kernel(const __grid_co
         __align__(16) TO x[32];
         // rows past M repeat the last one's residual; the tensor map cuts them
         lin_finish(a, min(m0 + lane, (long long)a.M - 1), n0 + 32 * c, v, x);
-        if (c == 0 || !ONE) {
+        if (!ONE || c % 2 == 0) {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the block before has been read
           __syncwarp();
         }
@@ -544,16 +551,16 @@ __global__ void __launch_bounds__(LP_THREADS, 1) lin_pair_kernel(const __grid_co
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           const uint4 w = *reinterpret_cast<const uint4*>(x + i * PER);
-          const unsigned at = row + ((((ONE ? 4 * c : 0) + i) ^ (lane & 7)) << 4);
+          const unsigned at = row + ((((ONE ? 4 * (c & 1) : 0) + i) ^ (lane & 7)) << 4);
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
         }
-        if (!ONE || c == 1 || n0 + 32 >= a.N) {
+        if (!ONE || c % 2 == 1 || n0 + 32 * c + 32 >= a.N) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
             asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
                              reinterpret_cast<unsigned long long>(&tmO)),
-                         "r"(n0 + (ONE ? 0 : 32 * c)), "r"((int)m0), "r"(obuf)
+                         "r"(n0 + 32 * (ONE ? c & ~1 : c)), "r"((int)m0), "r"(obuf)
                          : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
