@@ -182,6 +182,18 @@ template <typename TI, typename TO> TilePick tile_pick(int bn, unsigned xbytes, 
   return p;
 }
 
+struct PairPick {
+  PairKernel kern;
+  int threads;
+  size_t smem;
+};
+template <typename TI, typename TO> PairPick pair_pick(bool wide) {
+  using A = c4s::LpCfg<TO, 256>;
+  using B = c4s::LpCfg<TO, 128>;
+  return wide ? PairPick{c4s::lin_pair_kernel<TI, TO, 256>, A::THREADS, A::SMEM}
+              : PairPick{c4s::lin_pair_kernel<TI, TO, 128>, B::THREADS, B::SMEM};
+}
+
 // Launch in clusters of `cluster` CTAs along x.
 template <typename... P, typename... A>
 cudaError_t launch_cluster(void (*kern)(P...), dim3 grid, int cluster, int block, size_t smem, void* stream, A&&... args) {
@@ -220,17 +232,18 @@ cudaError_t launch_norm(const void* x, int M, int K, int64_t ldx, const float* g
                 K, vec, gamma, beta, aligned(gamma, beta), eps, (T*)y);
 }
 
-// The kernel for few rows. Sixteen warps a CTA where K is long.
+// The kernel for few rows.
 template <typename TI, typename TO>
 cudaError_t launch_few(const c4s_ctx* ctx, const void* x, long long ldx, const float* gamma, const float* beta, float eps,
                        bool norm, const void* w, long long ldw, const c4s::LinArgs& a, void* stream) {
   const bool xvec = ((uintptr_t)x & 15) == 0 && (ldx & 7) == 0;
-  const bool r16 = a.N >= 16 * ctx->num_sms, w16 = false;
-  auto kern = r16 ? (w16 ? c4s::lin_few_kernel<TI, TO, 16, 16> : c4s::lin_few_kernel<TI, TO, 16, 8>)
-                  : (w16 ? c4s::lin_few_kernel<TI, TO, 8, 16> : c4s::lin_few_kernel<TI, TO, 8, 8>);
+  const bool r16 = a.N >= 16 * ctx->num_sms;       // 16 rows of the weight a CTA where that leaves no SM without one
+  constexpr int NW = c4s::LF_WARPS;
+  auto kern = norm ? (r16 ? c4s::lin_few_kernel<TI, TO, 16, NW, true> : c4s::lin_few_kernel<TI, TO, 8, NW, true>)
+                   : (r16 ? c4s::lin_few_kernel<TI, TO, 16, NW, false> : c4s::lin_few_kernel<TI, TO, 8, NW, false>);
   const int R = r16 ? 16 : 8;
-  return launch(kern, dim3((unsigned)((a.N + R - 1) / R)), w16 ? 512 : 256, 0, stream, (const TI*)x, ldx, xvec, gamma,
-                beta, aligned(gamma, beta), eps, norm, (const TI*)w, ldw, a);
+  return launch(kern, dim3((unsigned)((a.N + R - 1) / R)), 32 * NW, 0, stream, (const TI*)x, ldx, xvec, gamma, beta,
+                aligned(gamma, beta), eps, (const TI*)w, ldw, a);
 }
 
 // Workspace of the attention: for every warp of the grid two parts of up to 8
@@ -421,19 +434,22 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
   }
   const bool f32 = out_dtype == C4S_FP32;
   const long long big = (long long)((M + 255) / 256) * ((N + 255) / 256);
+  const long long mid = (long long)((M + 255) / 256) * ((N + 127) / 128);
   CUtensorMap tx, tw;
-  if (big * 2 >= ctx->num_sms) {
-    // pairs of CTAs on 256 x 256 tiles where those fill the machine
+  if (big * 2 >= ctx->num_sms || (M > c4s::LN_BM && mid * 4 >= ctx->num_sms)) {
+    // pairs of CTAs on 256 x 256 tiles where those fill the machine, on 256 x 128 where those fill half of it
+    // (256 x 1280 -> 5120: 10.3 us by single CTAs on 160 tiles)
+    const bool wide = big * 2 >= ctx->num_sms;
     CUtensorMap to;
     memset(&to, 0, sizeof(to));
-    if (!encode_rows(&tx, dtype, d_x, K, M, ld_x * 2, 128) || !encode_rows(&tw, dtype, d_weight, K, N, ld_weight * 2, 128) ||
+    if (!encode_rows(&tx, dtype, d_x, K, M, ld_x * 2, 128) ||
+        !encode_rows(&tw, dtype, d_weight, K, N, ld_weight * 2, wide ? 128 : 64) ||
         (a.vec_out && !encode_rows(&to, out_dtype, d_out, N, M, ld_out * (long long)os, 32)))
       return fail(ctx, C4S_ERR_CUDA, "tensor map encoding failed");
-    const PairKernel k = dtype == C4S_BF16
-                             ? (f32 ? c4s::lin_pair_kernel<__nv_bfloat16, float> : c4s::lin_pair_kernel<__nv_bfloat16, __nv_bfloat16>)
-                             : (f32 ? c4s::lin_pair_kernel<__half, float> : c4s::lin_pair_kernel<__half, __half>);
-    e = launch_cluster(k, dim3((unsigned)(2 * std::min<long long>(big, ctx->num_sms / 2))), 2, f32 ? c4s::LpCfg<float>::THREADS : c4s::LpCfg<__half>::THREADS,
-                       f32 ? c4s::LpCfg<float>::SMEM : c4s::LpCfg<__half>::SMEM, stream, tx, tw, to, a);
+    const PairPick k = dtype == C4S_BF16 ? (f32 ? pair_pick<__nv_bfloat16, float>(wide) : pair_pick<__nv_bfloat16, __nv_bfloat16>(wide))
+                                         : (f32 ? pair_pick<__half, float>(wide) : pair_pick<__half, __half>(wide));
+    e = launch_cluster(k.kern, dim3((unsigned)(2 * std::min<long long>(wide ? big : mid, ctx->num_sms / 2))), 2,
+                       k.threads, k.smem, stream, tx, tw, to, a);
     return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "linear launch");
   }
   // tiles of 128 columns where they fill the machine, else of 64, and clusters of 2, 4 or 8 CTAs that share a

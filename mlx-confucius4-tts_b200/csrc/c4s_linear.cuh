@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
 // take tiles in turn, the accumulator is double-buffered in TMEM (2 x 256
 // columns), and the eight epilogue warps of each CTA finish a tile while the
 // next one's products run.
-constexpr unsigned LP_HALF = 128 * LN_BK * 2;      // 16 KB: a CTA's rows of x, or of W, of one k-block
+constexpr unsigned LP_HALF = 128 * LN_BK * 2;      // 16 KB: a CTA's rows of x of one k-block
 // A warp's block of the output on its way: 32 rows of 128 bytes (64 columns of
 // 16 bits, 32 of fp32), 16-byte pieces swizzled as the tensor map says. Written
 // by TMA, whole lines at once: 16-byte stores of one row a lane took 41 us of a
@@ -362,12 +362,16 @@ constexpr unsigned LP_HALF = 128 * LN_BK * 2;      // 16 KB: a CTA's rows of x, 
 constexpr unsigned LP_OUT = 32 * 128;
 // Sixteen epilogue warps hide the activation's latency best (GELU: 42.5 us
 // there, 45.2 with eight); fp32 outputs take more registers than those leave.
-template <typename TO>
+// BN 128: half the columns, for batches whose 256-wide tiles would leave SMs
+// without work.
+template <typename TO, int BN>
 struct LpCfg {
-  static constexpr int EPI = sizeof(TO) == 2 ? 16 : 8;         // epilogue warps
-  static constexpr int ST = EPI == 16 ? 5 : 6;                 // stages of the ring
+  static constexpr int EPI = sizeof(TO) == 2 && BN == 256 ? 16 : 8;        // epilogue warps
   static constexpr int THREADS = 64 + 32 * EPI;
-  static constexpr size_t SMEM = ST * 2 * (size_t)LP_HALF + EPI * (size_t)LP_OUT + 1024;
+  static constexpr unsigned WHALF = BN / 2 * LN_BK * 2;        // bytes of a CTA's rows of W of one k-block
+  static constexpr unsigned STAGE = LP_HALF + WHALF;
+  static constexpr int ST = BN == 256 ? (EPI == 16 ? 5 : 6) : 8;           // stages of the ring
+  static constexpr size_t SMEM = ST * (size_t)STAGE + EPI * (size_t)LP_OUT + 1024;
 };
 
 __device__ __forceinline__ unsigned map_rank(unsigned addr, unsigned rank) {
@@ -401,13 +405,14 @@ __device__ __forceinline__ void umma_commit_pair(unsigned long long* bar) {
       : "memory");
 }
 
-template <typename TI, typename TO>
-__global__ void __launch_bounds__(LpCfg<TO>::THREADS, 1) lin_pair_kernel(const __grid_constant__ CUtensorMap tmX,
+template <typename TI, typename TO, int BN>
+__global__ void __launch_bounds__(LpCfg<TO, BN>::THREADS, 1) lin_pair_kernel(const __grid_constant__ CUtensorMap tmX,
                                                                  const __grid_constant__ CUtensorMap tmW,
                                                                  const __grid_constant__ CUtensorMap tmO, LinArgs a) {
-  constexpr int ST = LpCfg<TO>::ST, EPI = LpCfg<TO>::EPI;
+  using Cfg = LpCfg<TO, BN>;
+  constexpr int ST = Cfg::ST, EPI = Cfg::EPI;
   constexpr unsigned BF = std::is_same<TI, __nv_bfloat16>::value ? 1u : 0u;
-  constexpr unsigned IDESC = (1u << 4) | (BF << 7) | (BF << 10) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+  constexpr unsigned IDESC = (1u << 4) | (BF << 7) | (BF << 10) | ((unsigned)(BN >> 3) << 17) | ((256u >> 4) << 24);
   extern __shared__ unsigned char lsm_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<unsigned long long>(lsm_raw) + 1023ull) & ~1023ull);
   __shared__ unsigned long long full[ST], empty[ST], acc_full[2], acc_empty[2];
@@ -417,7 +422,7 @@ __global__ void __launch_bounds__(LpCfg<TO>::THREADS, 1) lin_pair_kernel(const _
   const unsigned rank = blockIdx.x & 1u;           // in the pair
   const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
   const int KB = (a.K + LN_BK - 1) / LN_BK;
-  const int mt = (a.M + 255) / 256, nt = (a.N + 255) / 256;
+  const int mt = (a.M + 255) / 256, nt = (a.N + BN - 1) / BN;
   const long long tiles = (long long)mt * nt;
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
@@ -432,7 +437,7 @@ __global__ void __launch_bounds__(LpCfg<TO>::THREADS, 1) lin_pair_kernel(const _
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(512)
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(2 * BN)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
@@ -455,13 +460,13 @@ __global__ void __launch_bounds__(LpCfg<TO>::THREADS, 1) lin_pair_kernel(const _
     const unsigned s0 = smem_u32(ring), fb = smem_u32(full), eb = smem_u32(empty), lead = map_rank(fb, 0u);
     bool ok = true;
     for (long long t = pair; ok && t < tiles; t += pairs) {
-      const int m0 = (int)(t % mt) * 256 + (int)rank * 128, n0 = (int)(t / mt) * 256 + (int)rank * 128;
+      const int m0 = (int)(t % mt) * 256 + (int)rank * 128, n0 = (int)(t / mt) * BN + (int)rank * (BN / 2);
       for (int kb = 0; kb < KB; ++kb, ++it) {
         ok = mbar_wait_hot(eb + 8u * i, ph);
         if (!ok) break;
         if (elect_one()) {
-          const unsigned sx = s0 + (unsigned)i * 2 * LP_HALF, bar = lead + 8u * i;
-          if (rank == 0) mbar_expect_tx(fb + 8u * i, 4 * LP_HALF);
+          const unsigned sx = s0 + (unsigned)i * Cfg::STAGE, bar = lead + 8u * i;
+          if (rank == 0) mbar_expect_tx(fb + 8u * i, 2 * Cfg::STAGE);
           tma_load_pair(sx, &tmX, kb * LN_BK, m0, bar);
           tma_load_pair(sx + LP_HALF, &tmW, kb * LN_BK, n0, bar);
         }
@@ -492,10 +497,10 @@ __global__ void __launch_bounds__(LpCfg<TO>::THREADS, 1) lin_pair_kernel(const _
           if (!ok) { give_up(); break; }
           tc_fence_after();
           if (elect_one()) {
-            const unsigned long long xd = d0 + (unsigned)i * (2 * LP_HALF >> 4), wd = xd + (LP_HALF >> 4);
+            const unsigned long long xd = d0 + (unsigned)i * (Cfg::STAGE >> 4), wd = xd + (LP_HALF >> 4);
 #pragma unroll
             for (int kk = 0; kk < LN_BK / 16; ++kk)
-              umma_pair(tmem + (unsigned)(buf * 256), xd + 2ull * kk, wd + 2ull * kk, IDESC, (kb | kk) != 0 ? 1u : 0u);
+              umma_pair(tmem + (unsigned)(buf * BN), xd + 2ull * kk, wd + 2ull * kk, IDESC, (kb | kk) != 0 ? 1u : 0u);
             umma_commit_pair(&empty[i]);
           }
           __syncwarp();
@@ -506,19 +511,19 @@ __global__ void __launch_bounds__(LpCfg<TO>::THREADS, 1) lin_pair_kernel(const _
       }
     }
   } else {
-    constexpr int CW = 256 / (EPI / 4);               // columns of a warp
+    constexpr int CW = BN / (EPI / 4);               // columns of a warp
     const int q = warp & 3, cg = (warp - 2) >> 2;              // TMEM lane quarter, column group
-    const unsigned obuf = smem_u32(ring) + ST * 2 * LP_HALF + (unsigned)(warp - 2) * LP_OUT;
+    const unsigned obuf = smem_u32(ring) + ST * Cfg::STAGE + (unsigned)(warp - 2) * LP_OUT;
     int n = 0;
     for (long long t = pair; t < tiles; t += pairs, ++n) {
       const int buf = n & 1;
       const long long m0 = (t % mt) * 256 + rank * 128 + 32 * q;
-      const int n0 = (int)(t / mt) * 256 + CW * cg;
+      const int n0 = (int)(t / mt) * BN + CW * cg;
       const bool ok = mbar_wait_warp(&acc_full[buf], (unsigned)(n >> 1) & 1u);
       if (!ok) give_up();
       tc_fence_after();
       if (!__all_sync(FULL, ok) || abort_flag) break;
-      const unsigned taddr = tmem + ((unsigned)(32 * q) << 16) + (unsigned)(buf * 256 + CW * cg);
+      const unsigned taddr = tmem + ((unsigned)(32 * q) << 16) + (unsigned)(buf * BN + CW * cg);
       const bool tma = a.vec_out;                  // rows that a tensor map can name
       constexpr int PER = 16 / sizeof(TO), PIECES = 32 / PER;  // 16-byte pieces of a row's 32 columns
       constexpr bool ONE = PIECES == 4;            // both halves of the 64 columns make one block
@@ -576,7 +581,7 @@ __global__ void __launch_bounds__(LpCfg<TO>::THREADS, 1) lin_pair_kernel(const _
   cluster_wait();                                  // the pair's products and copies are done on both sides
   tc_fence_after();
   if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
 }
 
 // LayerNorm of the rows (nn.cpp:73-83: biased variance, (x - mean) / sqrt(var
@@ -658,14 +663,13 @@ __global__ void __launch_bounds__(LNORM_NT) lin_norm_kernel(const T* __restrict_
 // mean and variance while the weight is on its way (prefetched to L2 before the
 // kernel waits for the one before it), and x is normalised, and rounded as the
 // other forms round it, as it is loaded.
-constexpr int LF_ROWS = 8;
+constexpr int LF_ROWS = 8, LF_WARPS = 8;            // (sixteen warps: 9.9 us against 8.1 at 8 x 5120 -> 1280)
 
-template <typename TI, typename TO, int R, int WARPS>
+template <typename TI, typename TO, int R, int WARPS, bool NORM>
 __global__ void __launch_bounds__(32 * WARPS) lin_few_kernel(const TI* __restrict__ x, long long ldx, bool xvec,
                                                              const float* __restrict__ gamma,
                                                              const float* __restrict__ beta, bool gvec, float eps,
-                                                             bool norm, const TI* __restrict__ wt, long long ldw,
-                                                             LinArgs a) {
+                                                             const TI* __restrict__ wt, long long ldw, LinArgs a) {
   __shared__ float red[WARPS][LF_ROWS][R + 1];
   __shared__ float stat[LF_ROWS][2];               // mean, 1 / deviation
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -683,7 +687,24 @@ __global__ void __launch_bounds__(32 * WARPS) lin_few_kernel(const TI* __restric
   }
   grid_dep_wait();
   grid_dep_launch();
-  if (norm) {
+  constexpr int UN = R == 16 ? 2 : 4;              // pieces in flight: eight 16-byte loads a lane
+  constexpr int RH = R / 8;
+  const TI* w0 = wt + (long long)min(n0 + g, a.N - 1) * ldw;           // a row past N repeats the last one, unused
+  const TI* w1 = wt + (long long)min(n0 + g + 8, a.N - 1) * ldw;
+  uint4 wv[UN][2][RH];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = k0 + u * WARPS * 64 + h * 32 + t * 8;
+        const bool in = k < a.K;
+        wv[u][h][0] = in ? __ldcs(reinterpret_cast<const uint4*>(w0 + k)) : make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (RH == 2) wv[u][h][1] = in ? __ldcs(reinterpret_cast<const uint4*>(w1 + k)) : make_uint4(0u, 0u, 0u, 0u);
+      }
+  };
+  if constexpr (NORM) fetch(warp * 64);            // on its way while the norm's sums are taken
+  if constexpr (NORM) {
     for (int r = warp; r < a.M; r += WARPS) {
       const TI* xr = x + (long long)r * ldx;
       float s = 0.0f, q = 0.0f;
@@ -715,22 +736,9 @@ __global__ void __launch_bounds__(32 * WARPS) lin_few_kernel(const TI* __restric
   }
   float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   const bool mine = g < a.M;
-  const float mean = norm && mine ? stat[g][0] : 0.0f, rs = norm && mine ? stat[g][1] : 1.0f;
-  constexpr int UN = R == 16 ? 2 : 4;              // pieces in flight: eight 16-byte loads a lane
-  constexpr int RH = R / 8;
-  const TI* w0 = wt + (long long)min(n0 + g, a.N - 1) * ldw;           // a row past N repeats the last one, unused
-  const TI* w1 = wt + (long long)min(n0 + g + 8, a.N - 1) * ldw;
+  const float mean = NORM && mine ? stat[g][0] : 0.0f, rs = NORM && mine ? stat[g][1] : 1.0f;
   for (int k0 = warp * 64; k0 < a.K; k0 += UN * WARPS * 64) {
-    uint4 wv[UN][2][RH];
-#pragma unroll
-    for (int u = 0; u < UN; ++u)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = k0 + u * WARPS * 64 + h * 32 + t * 8;
-        const bool in = k < a.K;
-        wv[u][h][0] = in ? __ldcs(reinterpret_cast<const uint4*>(w0 + k)) : make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (RH == 2) wv[u][h][1] = in ? __ldcs(reinterpret_cast<const uint4*>(w1 + k)) : make_uint4(0u, 0u, 0u, 0u);
-      }
+    if (!NORM || k0 != warp * 64) fetch(k0);
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
@@ -740,7 +748,7 @@ __global__ void __launch_bounds__(32 * WARPS) lin_few_kernel(const TI* __restric
         if (k < a.K && mine) {
           TI v[8];
           load8c(x + (long long)g * ldx + k, xvec, v);
-          if (norm) {
+          if constexpr (NORM) {
             float ga[8], be[8];
             lin_gamma(gamma, beta, gvec, k, ga, be);
 #pragma unroll
