@@ -93,9 +93,15 @@ int kv_args(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* table, int64
   if (tstride < 0 || hstride < 0) return fail(ctx, C4S_ERR_INVALID, "negative stride");
   const uintptr_t es = dtype == C4S_FP32 ? 4 : 2;
   if (((uintptr_t)k | (uintptr_t)v) & (es - 1)) return fail(ctx, C4S_ERR_INVALID, "misaligned rows");
-  const long long units = (long long)cache->kv_heads * (cache->head_dim / 8);
-  if (T > 0x7fffffffLL * c4s::KV_NT / units - 1) return fail(ctx, C4S_ERR_CAPACITY, "too many tokens in one call");
-  grid = (unsigned)((T * units + c4s::KV_NT - 1) / c4s::KV_NT);
+  a.units = cache->kv_heads * (cache->head_dim / 8);
+  a.per_cta = std::max(1, std::min(c4s::KV_TOKS, c4s::KV_UNITS / a.units));
+  // few tokens: spread over the SMs
+  while (a.per_cta > 1 && (T + a.per_cta - 1) / a.per_cta < 4LL * ctx->num_sms) a.per_cta = (a.per_cta + 1) / 2;
+  const long long ctas = (T + a.per_cta - 1) / a.per_cta;
+  if (ctas > 0x7fffffffLL) return fail(ctx, C4S_ERR_CAPACITY, "too many tokens in one call");
+  grid = (unsigned)ctas;
+  a.udiv = c4s::page_div(a.units);
+  a.cdiv = c4s::page_div(cache->head_dim / 8);
   a.c = view(cache);
   a.table = table;
   a.table_ld = table_ld;

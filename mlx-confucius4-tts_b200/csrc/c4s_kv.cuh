@@ -7,22 +7,27 @@
 //     scale = (max - min) / n,  bias = min,  n = 2^bits - 1,
 //     code  = the integer nearest to n (x - min) / (max - min), ties to even,
 //     value = scale code + bias  (one fp32 FMA).
-// The quotient is formed in fp32, whose error here is below 2^-14 of a step
-// (255 times three roundings of 2^-24 and an approximate product); where it
-// falls within 2^-12 of a tie the decision is repeated in fp64, in which the
-// differences and the product are exact for 16-bit inputs. A group with a
-// non-finite element reads back as NaN throughout; a constant group has scale
-// 0 and reads back exactly.
+// The quotient is formed in fp32, whose error here is below 2^-13 of a step
+// (255 times the difference's rounding of 2^-24 and the approximate factor's
+// 2^-22); where it falls within 2^-12 of a tie the decision is repeated in
+// fp64, in which the differences and the product are exact for 16-bit inputs.
+// A group with a non-finite element reads back as NaN throughout; a constant
+// group has scale 0 and reads back exactly.
 //
 // One thread works 8 consecutive elements (16 B of the source) of a key row
 // and the same 8 of the value row: a group is 4 or 8 neighbouring lanes of one
-// warp, and its minimum and maximum take two or three shuffles. Both kernels
-// are bound by HBM: bytes of the source once, of the cache once.
+// warp, and its minimum and maximum take two or three shuffles. A CTA works a
+// few whole tokens; where each lies is found once, by one thread per token.
+// Both kernels are bound by HBM (the source's bytes once, the cache's once)
+// and close to it by instructions: integer codes are made and taken apart
+// with the float format's own bits, without conversions.
 #pragma once
 
 namespace c4s {
 
 constexpr int KV_NT = 256;
+constexpr int KV_UNITS = 1024;                     // units of 8 elements that a CTA works (at least one token, at most
+constexpr int KV_TOKS = 64;                        // KV_TOKS tokens)
 
 struct KvCache {
   unsigned char* k;
@@ -44,6 +49,8 @@ struct KvArgs {
   long long tstride, hstride;
   bool vec;                           // its rows are 16-byte aligned
   long long T;
+  int units, per_cta;                              // per token; tokens per CTA
+  PageDiv udiv, cdiv;                              // by the units of a token, of a head
   const long long* off;               // [B + 1] or null: token t is sequence t's
   const int* pos;                     // [B] position of a sequence's first token (< 0: skip it)
   unsigned* errflags;
@@ -94,43 +101,60 @@ __device__ __forceinline__ void store8(T* p, bool vec, const T (&x)[8]) {
   }
 }
 
-// Codes of 8 elements whose group has the extremes lo and hi.
+// Codes of 8 elements whose group has the extremes lo and hi, one a word. The
+// sum with 1.5 2^23 rounds to an integer (ties to even) and has it in its low bits.
 template <int BITS>
 __device__ __forceinline__ void kv_codes(const float (&x)[8], float lo, float hi, unsigned (&q)[8]) {
-  constexpr float n = (float)((1 << BITS) - 1);
-  const float inv = n / (hi - lo);
-  const bool plain = inv > 0.0f && inv < 3.0e38f;   // neither a range past fp32's, nor one near its smallest
+  constexpr float n = (float)((1 << BITS) - 1), R = 12582912.0f;
+  const float inv = __fdividef(n, hi - lo);
+  float off = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float t = (x[i] - lo) * inv;
-    float r = rintf(t);
-    if (!plain || fabsf(t - r) > 0.5f - 0x1p-12f)
-      r = hi > lo ? (float)rint(((double)x[i] - lo) * (double)n / ((double)hi - lo)) : 0.0f;
-    q[i] = (unsigned)fminf(fmaxf(r, 0.0f), n);
+    const float d = x[i] - lo, v = fmaf(d, inv, R);
+    q[i] = __float_as_uint(v);                     // the code in the low byte (the bits above are dropped)
+    off = fmaxf(off, fabsf(fmaf(d, inv, R - v)));
+  }
+  // near a tie, or a range past fp32's or near its smallest: decided in fp64
+  if (!(off < 0.5f - 0x1p-12f) || !(inv > 1e-30f && inv < 1e30f)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double r = hi > lo ? rint(((double)x[i] - lo) * (double)n / ((double)hi - lo)) : 0.0;
+      q[i] = (unsigned)fminf(fmaxf((float)r, 0.0f), n);
+    }
   }
 }
 
-// Where unit u (8 elements of a head of a token) lies; false: nothing to do.
-__device__ __forceinline__ bool kv_unit(const KvArgs& a, long long u, long long& tok, int& head, int& chunk, int& b,
-                                        int& page, int& slot, bool& bad) {
-  const int per_head = a.c.dim >> 3, per_tok = per_head * a.c.heads;
-  tok = u / per_tok;
-  const int r = (int)(u - tok * per_tok);
-  head = r / per_head;
-  chunk = r - head * per_head;
-  bad = false;
-  if (tok >= a.T) return false;
-  long long j = 0;
-  if (a.off) {
-    if (!token_sequence(a.off, a.B, tok, b)) return false;
-    j = tok - a.off[b];
-  } else {
-    b = (int)tok;
+// Where a CTA's tokens lie: offsets of a token's slot, of its scales (head 0);
+// found by one thread per token.
+struct KvPlace {
+  long long row, sb;
+  int state;                                       // 0: nothing to do, 1: a place, 2: no page
+};
+__device__ __forceinline__ void kv_places(const KvArgs& a, KvPlace* pl) {
+  const int i = threadIdx.x;
+  if (i < a.per_cta) {
+    const long long tok = (long long)blockIdx.x * a.per_cta + i;
+    KvPlace p{0, 0, 0};
+    int b = 0;
+    if (tok < a.T && (a.off == nullptr || token_sequence(a.off, a.B, tok, b))) {
+      if (a.off == nullptr) b = (int)tok;
+      const int p0 = a.pos[b];
+      int page, slot;
+      if (p0 >= 0) {
+        p.state = 2;
+        if (kv_locate(a.table + (long long)b * a.table_ld, a.max_pages, a.c.num_pages, a.c.page_size,
+                      p0 + (a.off ? tok - a.off[b] : 0), page, slot)) {
+          p.state = 1;
+          p.row = (long long)page * a.c.page_stride + (long long)slot * a.c.token_stride;
+          p.sb = (long long)page * a.c.sb_page_stride + (long long)slot * a.c.sb_token_stride;
+        } else {
+          atomicOr(a.errflags, C4S_DEVERR_KV_PAGE);
+        }
+      }
+    }
+    pl[i] = p;
   }
-  const int p0 = a.pos[b];
-  if (p0 < 0) return false;
-  bad = !kv_locate(a.table + (long long)b * a.table_ld, a.max_pages, a.c.num_pages, a.c.page_size, p0 + j, page, slot);
-  return true;
+  __syncthreads();
 }
 
 __device__ __forceinline__ long long kv_row(const KvCache& c, int page, int head, int slot) {
@@ -148,40 +172,38 @@ __device__ __forceinline__ void kv_put(const T (&x)[8], unsigned char* row, unsi
   if constexpr (BITS == 16) {
     if (live) store8(reinterpret_cast<T*>(row) + 8 * chunk, true, x);
   } else {
-    float f[8], lo = INFINITY, hi = -INFINITY;
-    bool odd = false;
+    float f[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] = Cvt<T>::f(x[i]);
-      lo = fminf(lo, f[i]);
-      hi = fmaxf(hi, f[i]);
-      odd |= !(fabsf(f[i]) < INFINITY);
-    }
-    if (odd) hi = INFINITY;
+    for (int i = 0; i < 8; ++i) f[i] = Cvt<T>::f(x[i]);
+    float lo = fminf(fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), fminf(fminf(f[4], f[5]), fminf(f[6], f[7])));
+    float hi = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+    // a NaN among them is in no minimum or maximum, but in their sum of differences from themselves
+    float odd = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) odd += f[i] - f[i];
+    if (!(odd == 0.0f)) hi = INFINITY;
     for (int o = 1; o < glanes; o <<= 1) {
       lo = fminf(lo, __shfl_xor_sync(FULL, lo, o));
       hi = fmaxf(hi, __shfl_xor_sync(FULL, hi, o));
     }
-    const bool fine = hi < INFINITY;
     unsigned q[8];
     kv_codes<BITS>(f, lo, hi, q);
     if (!live) return;
     constexpr float n = (float)((1 << BITS) - 1);
     if ((chunk & (glanes - 1)) == 0) {
-      const float d = hi - lo;
+      const float d = hi - lo, nan = __int_as_float(0x7fc00000);
       const float scale = d < INFINITY ? d / n : hi / n - lo / n;
-      *reinterpret_cast<float2*>(sb + 8 * (chunk / glanes)) =
-          fine ? make_float2(scale, lo) : make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
+      *reinterpret_cast<float2*>(sb + 8 * (chunk / glanes)) = hi < INFINITY ? make_float2(scale, lo) : make_float2(nan, nan);
     }
     if constexpr (BITS == 8) {
       uint2 w;
-      w.x = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
-      w.y = q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24;
+      w.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+      w.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
       *reinterpret_cast<uint2*>(row + 8 * chunk) = w;
     } else {
       unsigned w = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w |= q[i] << (4 * i);
+      for (int i = 0; i < 8; ++i) w |= (q[i] & 15u) << (4 * i);
       *reinterpret_cast<unsigned*>(row + 4 * chunk) = w;
     }
   }
@@ -189,31 +211,33 @@ __device__ __forceinline__ void kv_put(const T (&x)[8], unsigned char* row, unsi
 
 template <typename T, int BITS>
 __global__ void __launch_bounds__(KV_NT) kv_write_kernel(KvArgs a) {
+  __shared__ KvPlace pl[KV_TOKS];
   grid_dep_wait();                                 // the projection that made the new rows
   grid_dep_launch();
-  const long long u = (long long)blockIdx.x * KV_NT + threadIdx.x;
-  long long tok;
-  int head, chunk, b, page = 0, slot = 0;
-  bool bad;
-  const bool mine = kv_unit(a, u, tok, head, chunk, b, page, slot, bad);
-  if (mine && bad && head == 0 && chunk == 0) atomicOr(a.errflags, C4S_DEVERR_KV_PAGE);
-  const bool live = mine && !bad;
-  T xk[8], xv[8];
+  kv_places(a, pl);
+  const int glanes = a.c.group >> 3, total = a.per_cta * a.units;
+  for (int u0 = 0; u0 < total; u0 += KV_NT) {
+    const int u = u0 + threadIdx.x;
+    const int tk = min(page_of(a.udiv, u), a.per_cta - 1);
+    const int r = u - tk * a.units, head = page_of(a.cdiv, r), chunk = r - head * (a.c.dim >> 3);
+    const bool live = u < total && pl[tk].state == 1;
+    T xk[8], xv[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) xk[i] = xv[i] = Cvt<T>::t(0.0f);
-  if (live) {
-    const long long s = tok * a.tstride + (long long)head * a.hstride + 8 * chunk;
-    load8(static_cast<const T*>(a.k) + s, a.vec, xk);
-    load8(static_cast<const T*>(a.v) + s, a.vec, xv);
+    for (int i = 0; i < 8; ++i) xk[i] = xv[i] = Cvt<T>::t(0.0f);
+    if (live) {
+      const long long s = ((long long)blockIdx.x * a.per_cta + tk) * a.tstride + (long long)head * a.hstride + 8 * chunk;
+      load8(static_cast<const T*>(a.k) + s, a.vec, xk);
+      load8(static_cast<const T*>(a.v) + s, a.vec, xv);
+    }
+    const long long row = live ? pl[tk].row + (long long)head * a.c.head_stride : 0;
+    const long long sb = BITS != 16 && live ? pl[tk].sb + (long long)head * a.c.sb_head_stride : 0;
+    kv_put<T, BITS>(xk, a.c.k + row, a.c.k_sb + sb, chunk, glanes, live);
+    kv_put<T, BITS>(xv, a.c.v + row, a.c.v_sb + sb, chunk, glanes, live);
   }
-  const long long row = live ? kv_row(a.c, page, head, slot) : 0;
-  const long long sb = BITS != 16 && live ? kv_sb(a.c, page, head, slot) : 0;
-  const int glanes = a.c.group >> 3;
-  kv_put<T, BITS>(xk, a.c.k + row, a.c.k_sb + sb, chunk, glanes, live);
-  kv_put<T, BITS>(xv, a.c.v + row, a.c.v_sb + sb, chunk, glanes, live);
 }
 
-// TC: type of 16-bit cache rows (unused for codes); TO: type of the output.
+// 8 elements of a row's values. TC: type of 16-bit cache rows (unused for
+// codes); TO: type of the output. A code's byte becomes the float 2^23 + code.
 template <typename TC, typename TO, int BITS>
 __device__ __forceinline__ void kv_get(const unsigned char* row, const unsigned char* sb, int chunk, int glanes,
                                        TO (&y)[8]) {
@@ -224,42 +248,49 @@ __device__ __forceinline__ void kv_get(const unsigned char* row, const unsigned 
     for (int i = 0; i < 8; ++i) y[i] = Cvt<TO>::t(Cvt<TC>::f(x[i]));
   } else {
     const float2 p = *reinterpret_cast<const float2*>(sb + 8 * (chunk / glanes));
+    uint2 w;
     if constexpr (BITS == 8) {
-      const uint2 w = __ldcs(reinterpret_cast<const uint2*>(row + 8 * chunk));
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        y[i] = Cvt<TO>::t(fmaf(p.x, (float)(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xffu), p.y));
+      w = __ldcs(reinterpret_cast<const uint2*>(row + 8 * chunk));
     } else {
-      const unsigned w = __ldcs(reinterpret_cast<const unsigned*>(row + 4 * chunk));
+      const unsigned v = __ldcs(reinterpret_cast<const unsigned*>(row + 4 * chunk));
+      w = make_uint2(v & 0x0f0f0f0fu, (v >> 4) & 0x0f0f0f0fu);       // even, odd elements
+    }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = Cvt<TO>::t(fmaf(p.x, (float)((w >> (4 * i)) & 0xfu), p.y));
+    for (int i = 0; i < 8; ++i) {
+      const unsigned word = BITS == 8 ? (i < 4 ? w.x : w.y) : (i & 1 ? w.y : w.x);
+      const unsigned sel = 0x7440u + (BITS == 8 ? (i & 3) : (i >> 1));
+      const float f = __uint_as_float(__byte_perm(word, 0x4b000000u, sel)) - 8388608.0f;
+      y[i] = Cvt<TO>::t(fmaf(p.x, f, p.y));
     }
   }
 }
 
 template <typename TC, typename TO, int BITS>
 __global__ void __launch_bounds__(KV_NT) kv_read_kernel(KvArgs a) {
+  __shared__ KvPlace pl[KV_TOKS];
   grid_dep_wait();                                 // the writes of earlier kernels
   grid_dep_launch();
-  const long long u = (long long)blockIdx.x * KV_NT + threadIdx.x;
-  long long tok;
-  int head, chunk, b, page = 0, slot = 0;
-  bool bad;
-  if (!kv_unit(a, u, tok, head, chunk, b, page, slot, bad)) return;
-  TO yk[8], yv[8];
-  if (bad) {
-    if (head == 0 && chunk == 0) atomicOr(a.errflags, C4S_DEVERR_KV_PAGE);
+  kv_places(a, pl);
+  const int total = a.per_cta * a.units;
+  for (int u = threadIdx.x; u < total; u += KV_NT) {
+    const int tk = page_of(a.udiv, u);
+    const int r = u - tk * a.units, head = page_of(a.cdiv, r), chunk = r - head * (a.c.dim >> 3);
+    const int state = pl[tk].state;
+    if (state == 0) continue;
+    TO yk[8], yv[8];
+    if (state == 2) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) yk[i] = yv[i] = Cvt<TO>::t(0.0f);
-  } else {
-    const long long row = kv_row(a.c, page, head, slot);
-    const long long sb = BITS != 16 ? kv_sb(a.c, page, head, slot) : 0;
-    kv_get<TC, TO, BITS>(a.c.k + row, a.c.k_sb + sb, chunk, a.c.group >> 3, yk);
-    kv_get<TC, TO, BITS>(a.c.v + row, a.c.v_sb + sb, chunk, a.c.group >> 3, yv);
+      for (int i = 0; i < 8; ++i) yk[i] = yv[i] = Cvt<TO>::t(0.0f);
+    } else {
+      const long long row = pl[tk].row + (long long)head * a.c.head_stride;
+      const long long sb = BITS != 16 ? pl[tk].sb + (long long)head * a.c.sb_head_stride : 0;
+      kv_get<TC, TO, BITS>(a.c.k + row, a.c.k_sb + sb, chunk, a.c.group >> 3, yk);
+      kv_get<TC, TO, BITS>(a.c.v + row, a.c.v_sb + sb, chunk, a.c.group >> 3, yv);
+    }
+    const long long s = ((long long)blockIdx.x * a.per_cta + tk) * a.tstride + (long long)head * a.hstride + 8 * chunk;
+    store8(static_cast<TO*>(const_cast<void*>(a.k)) + s, a.vec, yk);
+    store8(static_cast<TO*>(const_cast<void*>(a.v)) + s, a.vec, yv);
   }
-  const long long s = tok * a.tstride + (long long)head * a.hstride + 8 * chunk;
-  store8(static_cast<TO*>(const_cast<void*>(a.k)) + s, a.vec, yk);
-  store8(static_cast<TO*>(const_cast<void*>(a.v)) + s, a.vec, yv);
 }
 
 }  // namespace c4s
