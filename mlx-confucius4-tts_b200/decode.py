@@ -13,9 +13,10 @@ that on the device:
     decode_step      stop-token check, history and latent append, next
                      embeddings (c4s_decode_step)
 
-The GPT-2 forward pass itself (the KV-cached transformer) is the caller's: it
-is a function next_embeddings -> hidden states handed to run(). Nothing crosses
-to the host per step except, every `poll_every` steps, the count of finished
+The forward pass itself (the KV-cached transformer) is a function
+next_embeddings -> hidden states handed to run(): the caller's own, or a
+GPT2Stack, which runs GPT-2 blocks over a paged key-value cache with the
+context's operators. Nothing crosses to the host per step except, every `poll_every` steps, the count of finished
 streams. Rows that finish keep their RNG state and history; once every row is
 done the loop stops (at most poll_every - 1 steps later, steps in which no row
 is active and nothing changes).
@@ -116,3 +117,92 @@ class DecodeLoop:
             n = int(lens[b])
             out.append((hist[b, :n].copy(), None if lat is None else lat[b, :n].copy()))
         return out
+
+
+class GPT2Stack:
+    """GPT-2 blocks with a paged key-value cache, one token per stream and call:
+    the `forward` of DecodeLoop.run (gpt2.cpp's blocks with their cache). Per block
+
+        qkv = linear(LN1(h))           c4s_linear, the norm in the same call
+        cache <- k, v                  c4s_kv_write, quantized as written for bits 8 or 4
+        a = attention(q, cache)        c4s_paged_attention
+        h = h + linear(a)              c4s_linear, the residual in its epilogue
+        h = h + linear(gelu(linear(LN2(h))))
+
+    with the residual stream in bf16, as the head takes it. All state (lengths,
+    page table, caches, buffers) lives on the device; a call reads nothing back
+    and allocates nothing, so a step can be captured into a CUDA graph.
+
+    layers       one dict per block of bf16 weights, out x in (a checkpoint's
+                 Conv1D weights transposed), fp32 biases (or None) and norms:
+                 attn_w [3d, d], attn_b, proj_w [d, d], proj_b, fc_w [m, d],
+                 fc_b, out_w [d, m], out_b, ln1_g, ln1_b, ln2_g, ln2_b [d]
+    heads        d / heads must be 64, 96 or 128
+    positions    places per stream (prompt and generated tokens)
+    bits, group  of the cache: 16 (bf16 rows), 8 or 4 (codes)
+    active       DecodeLoop.active: streams that stopped are neither written nor
+                 attended to (their hidden states are not used)
+    """
+
+    def __init__(self, ctx, layers, heads: int, B: int, positions: int, bits: int = 16, group: int = 64,
+                 page_size: int = 64, active=None, eps: float = 1e-5):
+        import torch
+        from .block import KVCache
+        self.ctx, self.layers, self.heads, self.B, self.eps, self.active = ctx, layers, heads, B, eps, active
+        self.d = layers[0]["attn_w"].shape[1]
+        if self.d % heads:
+            raise ValueError("the width must be a multiple of the heads")
+        dev, hd, bf = layers[0]["attn_w"].device, self.d // heads, torch.bfloat16
+        per = -(-positions // page_size)
+        self.positions = positions
+        self.table = torch.arange(B * per, dtype=torch.int32, device=dev).view(B, per)
+        self.caches = [KVCache.empty(B * per, page_size, heads, hd, bits=bits, group=group, device=dev) for _ in layers]
+        self.lens = torch.zeros(B, dtype=torch.int32, device=dev)      # tokens cached
+        self.pos = torch.zeros(B, dtype=torch.int32, device=dev)       # of this step's tokens, -1: stopped
+        self.seen = torch.zeros(B, dtype=torch.int32, device=dev)      # positions to attend to, 0: stopped
+        self.h = torch.empty((B, self.d), dtype=bf, device=dev)
+        self.qkv = torch.empty((B, 3, heads, hd), dtype=bf, device=dev)
+        self.att = torch.empty((B, heads, hd), dtype=bf, device=dev)
+        self.mlp = torch.empty((B, layers[0]["fc_w"].shape[0]), dtype=bf, device=dev)
+        self.norm = torch.empty((B, self.d), dtype=bf, device=dev)
+        self.work = ctx.attention_workspace(B, heads, hd)
+
+    def write_prompt(self, layer: int, k, v, tok_off):
+        """Caches the prompts' keys and values of one block, [T, heads, head_dim],
+        stream b's tokens tok_off[b]:tok_off[b+1] from position 0; follow the last
+        block's by prompt_done."""
+        self.ctx.kv_write(self.caches[layer], self.table, k, v, self._zeros(), tok_off=tok_off)
+
+    def _zeros(self):
+        return self.pos.zero_()
+
+    def prompt_done(self, tok_off):
+        """The prompts of every block are cached: their lengths count."""
+        self.lens.copy_(tok_off[1:] - tok_off[:-1])
+
+    def __call__(self, emb, step=None):
+        """One token per stream: emb [B, d] bf16 (or its bits) -> hidden states [B, d] as int16 bits, as
+        DecodeLoop hands them on. The result is overwritten by the next call."""
+        import torch
+        c, B, d = self.ctx, self.B, self.d
+        self.h.copy_(emb if emb.dtype == torch.bfloat16 else emb.view(torch.bfloat16))
+        self.pos.copy_(self.lens)
+        if self.active is None:
+            self.lens += 1
+            self.seen.copy_(self.lens)
+        else:
+            on = self.active.to(torch.int32)
+            self.lens += on
+            torch.mul(self.lens, on, out=self.seen)
+            torch.sub((self.pos + 1) * on, 1, out=self.pos)
+        h, qkv, att = self.h, self.qkv, self.att
+        for p, cache in zip(self.layers, self.caches):
+            c.linear(h, p["attn_w"], p.get("attn_b"), layer_norm=True, gamma=p["ln1_g"], beta=p["ln1_b"], eps=self.eps,
+                     norm_out=self.norm, out=qkv.view(B, 3 * d))
+            c.kv_write(cache, self.table, qkv[:, 1], qkv[:, 2], self.pos)
+            c.paged_attention(qkv[:, 0], cache, self.table, self.seen, out=att, work=self.work)
+            c.linear(att.view(B, d), p["proj_w"], p.get("proj_b"), residual=h, out=h)
+            c.linear(h, p["fc_w"], p.get("fc_b"), act="gelu", layer_norm=True, gamma=p["ln2_g"], beta=p["ln2_b"],
+                     eps=self.eps, norm_out=self.norm, out=self.mlp)
+            c.linear(self.mlp, p["out_w"], p.get("out_b"), residual=h, out=h)
+        return h.view(torch.int16)

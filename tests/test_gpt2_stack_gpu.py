@@ -1,0 +1,170 @@
+"""DecodeLoop with GPT2Stack as its forward pass: the block's operators as they
+are used together.
+
+Every operator call of a decode is recorded with what it was given, checked
+against fp64 on those inputs (the bounds of test_linear_gpu.py and
+test_block_gpu.py), and the flow between the calls is the blocks' own: what a
+call is given is what an earlier one left. A step captured into a graph and
+replayed gives the eager bits, and a prompt written at once gives the cache
+that the same tokens give one by one.
+"""
+import numpy as np
+import pytest
+
+from conftest import load_c4s
+from test_block_gpu import check_attention
+from test_linear_gpu import check
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+DEV = "cuda:0"
+BF = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def c4s():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return load_c4s()
+
+
+class Recorder:
+    """Passes operator calls on, checks each of them."""
+
+    def __init__(self, ctx, c4s):
+        self.ctx, self.c4s, self.calls = ctx, c4s, []
+
+    def __getattr__(self, name):
+        return getattr(self.ctx, name)
+
+    def linear(self, x, w, bias=None, **kw):
+        x0 = x.clone()
+        res = kw.get("residual")
+        res = None if res is None else res.clone()
+        out = self.ctx.linear(x, w, bias, **kw)
+        check(self.ctx, x0, w, out, bias=bias, act=kw.get("act", "none"), residual=res,
+              layer_norm=kw.get("layer_norm", False), gamma=kw.get("gamma"), beta=kw.get("beta"), eps=kw.get("eps", 1e-5))
+        self.calls.append(("linear", x0, out.clone()))
+        return out
+
+    def kv_write(self, cache, table, k, v, pos, **kw):
+        self.ctx.kv_write(cache, table, k, v, pos, **kw)
+        on = pos >= 0
+        p = pos.clamp(min=0)
+        rk, rv = self.ctx.kv_read(cache, table, p, dtype=torch.float32)
+        for got, new in ((rk, k), (rv, v)):
+            if cache.bits == 16:
+                assert torch.equal(got[on], new[on].float())
+            else:
+                g = new.float().unflatten(-1, (-1, cache.struct.group))
+                step = (g.amax(-1) - g.amin(-1)) / (2 ** cache.bits - 1)
+                err = (got - new.float()).abs().unflatten(-1, (-1, cache.struct.group)).amax(-1)
+                size = g.abs().amax(-1)
+                assert torch.all((err <= step / 2 + size * 2.0 ** -20)[on])
+        self.calls.append(("write", k.clone(), None))
+
+    def paged_attention(self, q, cache, table, lens, **kw):
+        out = self.ctx.paged_attention(q, cache, table, lens, **kw)
+        check_attention(self.ctx, self.c4s, q, cache, table, lens.tolist(), None, cache.head_dim ** -0.5, out)
+        self.calls.append(("attention", q.clone(), out.clone()))
+        return out
+
+
+def model(d, m, n_layers, V, positions, g):
+    r = lambda *s: torch.randn(s, generator=g, device=DEV)
+    layers = [dict(attn_w=(r(3 * d, d) * d ** -0.5).to(BF), attn_b=r(3 * d) * 0.1,
+                   proj_w=(r(d, d) * d ** -0.5).to(BF), proj_b=r(d) * 0.1,
+                   fc_w=(r(m, d) * d ** -0.5).to(BF), fc_b=r(m) * 0.1,
+                   out_w=(r(d, m) * m ** -0.5).to(BF), out_b=None,
+                   ln1_g=1 + 0.1 * r(d), ln1_b=0.1 * r(d), ln2_g=1 + 0.1 * r(d), ln2_b=0.1 * r(d))
+              for _ in range(n_layers)]
+    head = dict(weight=(r(V, d) * 0.3).to(BF).view(torch.int16), bias=r(V) * 0.5, gamma=1 + 0.1 * r(d), beta=0.1 * r(d))
+    emb, pos = r(V, d).to(BF).view(torch.int16), (0.3 * r(positions, d)).to(BF).view(torch.int16)
+    return layers, head, emb, pos
+
+
+@pytest.mark.parametrize("B,bits,group", [(1, 16, 64), (5, 8, 64), (20, 4, 32)])
+def test_decode_through_the_blocks(c4s, B, bits, group):
+    d, m, V, steps = 256, 512, 300, 24
+    g = torch.Generator(device=DEV).manual_seed(B)
+    layers, head, emb, pos = model(d, m, 2, V, steps + 1, g)
+    head["bias"][V - 1] = 6.0 if B > 1 else -9.0       # streams stop at different steps
+    ctx = c4s.SamplingContext(max_vocab=V, device=0, max_rows=32)
+    params = c4s.workloads.make_params(B, temperature=0.9, top_k=20, top_p=0.9, repetition_penalty=1.3)
+    loop = c4s.decode.DecodeLoop(ctx, B, head, emb, pos, params, seed=5, max_new_tokens=steps, stop_token=V - 1)
+    rec = Recorder(ctx, c4s)
+    stack = c4s.decode.GPT2Stack(rec, layers, 4, B, steps + 4, bits=bits, group=group, page_size=8, active=loop.active)
+    start = torch.randn((B, d), generator=g, device=DEV).to(BF).view(torch.int16)
+    hidden = stack(start)
+    res = loop.run(stack, hidden)
+    assert ctx.status()[0] == 0
+    counts = [len(r[0]) for r in res]
+    assert (stack.lens.cpu().numpy() >= np.array(counts)).all()
+    if B > 1:
+        assert min(counts) < steps
+    kinds = [c[0] for c in rec.calls]
+    assert kinds[:6] == ["linear", "write", "attention", "linear", "linear", "linear"] and len(kinds) % 12 == 0
+    # the flow of the first block of the first call
+    c = rec.calls
+    assert torch.equal(c[0][1], start.view(BF))
+    qkv = c[0][2].view(B, 3, 4, d // 4)
+    assert torch.equal(c[1][1], qkv[:, 1]) and torch.equal(c[2][1], qkv[:, 0])
+    assert torch.equal(c[3][1], c[2][2].view(B, d)) and torch.equal(c[4][1], c[3][2]) and torch.equal(c[5][1], c[4][2])
+    assert torch.equal(c[6][1], c[5][2])
+
+
+def test_captured_step(c4s):
+    """A step of the blocks replayed from a graph gives the eager step's bits, while the caches grow."""
+    B, d, steps = 3, 128, 20
+    g = torch.Generator(device=DEV).manual_seed(3)
+    layers, _, _, _ = model(d, 256, 2, 50, 10, g)
+    ctx = c4s.SamplingContext(max_vocab=64, device=0, max_rows=4)
+    a = c4s.decode.GPT2Stack(ctx, layers, 2, B, steps + 4, bits=8, page_size=4)
+    b = c4s.decode.GPT2Stack(ctx, layers, 2, B, steps + 4, bits=8, page_size=4)
+    x = torch.randn((B, d), generator=g, device=DEV).to(BF)
+    xin = x.clone()
+    b(xin)
+    b.lens.zero_()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = b(xin)
+    b.lens.zero_()
+    for s in range(steps):
+        want = a(x).view(BF).clone()
+        xin.copy_(x)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(BF), want), s
+        x = want
+    assert a.lens.tolist() == [steps] * B == b.lens.tolist()
+    assert ctx.status()[0] == 0
+
+
+def test_prompt_at_once_and_token_by_token(c4s):
+    B, heads, hd = 4, 2, 64
+    g = torch.Generator(device=DEV).manual_seed(4)
+    layers, _, _, _ = model(heads * hd, 128, 1, 50, 10, g)
+    ctx = c4s.SamplingContext(max_vocab=64, device=0, max_rows=4)
+    lens = [3, 0, 9, 5]
+    off = torch.tensor([0] + list(np.cumsum(lens)), device=DEV)
+    k = torch.randn((17, heads, hd), generator=g, device=DEV).to(BF)
+    v = torch.randn((17, heads, hd), generator=g, device=DEV).to(BF)
+    a = c4s.decode.GPT2Stack(ctx, layers, heads, B, 16, bits=8, page_size=4)
+    b = c4s.decode.GPT2Stack(ctx, layers, heads, B, 16, bits=8, page_size=4)
+    a.write_prompt(0, k, v, off)
+    a.prompt_done(off)
+    assert a.lens.tolist() == lens
+    for i in range(max(lens)):
+        on = [n > i for n in lens]
+        idx = torch.tensor([int(off[j]) + i if on[j] else 0 for j in range(B)], device=DEV)
+        p = torch.tensor([i if on[j] else -1 for j in range(B)], dtype=torch.int32, device=DEV)
+        ctx.kv_write(b.caches[0], b.table, k[idx], v[idx], p)
+    for x, y in ((a.caches[0].k, b.caches[0].k), (a.caches[0].v, b.caches[0].v), (a.caches[0].k_sb, b.caches[0].k_sb),
+                 (a.caches[0].v_sb, b.caches[0].v_sb)):
+        assert torch.equal(x, y)
+    x = torch.randn((B, heads * hd), generator=g, device=DEV).to(BF)
+    b.prompt_done(off)
+    assert torch.equal(a(x), b(x))
