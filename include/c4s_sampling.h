@@ -290,9 +290,9 @@ int c4s_kv_read(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* d_page_t
  * Lengths are read on the device, so the call can be captured while they
  * grow. Scores, softmax and sums are fp32; P is not rounded to 16 bits.
  * d_work: caller-owned device workspace, 16-byte aligned, of at least
- * c4s_attention_workspace(ctx, B, q_heads, head_dim) bytes, zeroed once
- * before its first use (each call leaves it ready for the next); calls that
- * may overlap in time need workspaces of their own.
+ * c4s_attention_workspace(ctx, B, q_heads, head_dim) bytes (contents need no
+ * initialisation and mean nothing afterwards); calls that may overlap in time
+ * need workspaces of their own.
  * Replaces the fused attention call of gpt2.cpp's decode step.             */
 int64_t c4s_attention_workspace(c4s_ctx* ctx, int32_t B, int32_t q_heads, int32_t head_dim);
 int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* d_page_table, int64_t table_ld,

@@ -49,13 +49,14 @@ def _torch():
 
 
 _bind = None
+_KINDS = {}                     # torch type -> c4s_dtype, filled with the binding
 
 
 def binding():
     """The compiled binding (csrc/c4s_bind.cpp, built by __graft_entry__.build())."""
     global _bind
     if _bind is None:
-        _torch()
+        torch = _torch()
         path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_c4s.so")
         if not os.path.exists(path):
             raise RuntimeError(f"c4s binding not built: {path} is missing "
@@ -65,6 +66,7 @@ def binding():
         spec.loader.exec_module(mod)
         from .sampling import C4SError
         mod.set_error(C4SError)
+        _KINDS.update({torch.bfloat16: BF16, torch.float16: FP16, torch.float32: FP32})
         _bind = mod
     return _bind
 
@@ -225,29 +227,28 @@ class BlockOps:
             return self._on_stream(stream, self.kv_read, cache, page_table, pos, tok_off, total, dtype, k_out, v_out)
         if (k_out is None) != (v_out is None):
             raise ValueError("k_out and v_out go together")
-        if k_out is None:
-            torch = _torch()
-            if total is None:
-                if tok_off is not None:
-                    raise ValueError("total is needed with tok_off")
-                total = page_table.shape[0]
-            if dtype is None:
-                dtype = torch.bfloat16 if cache.bits != 16 else cache.k.dtype
-            s = cache.struct
-            # one allocation: keys, then values
-            k_out, v_out = torch.empty((2, total, s.kv_heads, s.head_dim), dtype=dtype, device=self.device).unbind(0)
-        binding().kv(self._handle(), self.device.index or 0, cache.address, cache.device_index, page_table, k_out, v_out,
-                     pos, tok_off, False)
-        return k_out, v_out
+        if k_out is not None:
+            binding().kv(self._handle(), self.device.index or 0, cache.address, cache.device_index, page_table, k_out,
+                         v_out, pos, tok_off, False)
+            return k_out, v_out
+        if total is None:
+            if tok_off is not None:
+                raise ValueError("total is needed with tok_off")
+            total = page_table.shape[0]
+        bind = binding()
+        if dtype is not None and dtype not in _KINDS:
+            raise TypeError(f"{dtype} is not supported")
+        return bind.kv_read(self._handle(), self.device.index or 0, cache.address, cache.device_index, page_table,
+                                 pos, tok_off, total, _KINDS[dtype] if dtype is not None else -1)
 
     def attention_workspace(self, batch: int, q_heads: int, head_dim: int, stream=None):
-        """A zeroed workspace for paged_attention. Keep one per stream (or captured graph)."""
+        """A workspace for paged_attention. Keep one per stream (or captured graph)."""
         if stream is not None:
             return self._on_stream(stream, self.attention_workspace, batch, q_heads, head_dim)
         n = self.lib.c4s_attention_workspace(self._h, batch, q_heads, head_dim)
         if n < 0:
             self._check(int(n), "c4s_attention_workspace")
-        return _torch().zeros(n, dtype=_torch().uint8, device=self.device)
+        return _torch().empty(n, dtype=_torch().uint8, device=self.device)
 
     def paged_attention(self, q, cache: KVCache, page_table, lens, start=None, scale: float | None = None, out=None,
                         work=None, stream=None):

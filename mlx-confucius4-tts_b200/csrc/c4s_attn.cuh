@@ -14,8 +14,11 @@
 // to keep enough of those rows in flight.
 //   * The tiles of all (sequence, head) segments form one list, split evenly
 //     over all warps of the grid (c4s_kvidx.cuh), so that one long sequence,
-//     many short ones and ragged batches all fill the machine, and lengths are
-//     read on the device only (the call can be captured).
+//     many short ones and ragged batches all fill the machine; a second kernel
+//     joins the segments that a share's border cuts. Where segments are short,
+//     a CTA takes each and its warps meet in shared memory: one launch, no
+//     prefix sums. Lengths are read on the device only (the call can be
+//     captured); which of the two runs goes by what the page table can name.
 //   * Each warp runs its own pipeline of ATT stages of cp.async copies into
 //     its own part of shared memory: no barrier of the CTA in the loop. Rows
 //     are found through the page table by the lane that owns the token, one
@@ -34,13 +37,18 @@
 //     bias act on the scores and on P: q.k = scale (q.code) + bias sum(q),
 //     p v = (p scale) code + p bias, per group (of codes centred on zero). q is scaled by a power of two
 //     into fp16's upper range, p scale by the largest scale seen so far.
+//
+// Measured on one B200 (graph, warm; GB/s of the bytes that cannot be done
+// without): 256 ragged sequences of up to 1500, 20 heads of 64, bf16 156 us
+// (6180), 2 x 50001 x 8 heads of 128, fp16 72 us (5730), 64 of up to 1600 in
+// 8-bit codes 43 us (3410), one of 700 5.9 us.
 #pragma once
 
 namespace c4s {
 
 constexpr int ATT_CTAS = 2;                        // per SM: what registers and shared memory are sized for
 constexpr int ATT_MAXB = 256;                      // sequences per launch (their prefix sums in shared memory)
-constexpr int ATT_JOIN_NT = 128;
+constexpr int ATT_JOIN_NT = 256;
 
 struct AttnArgs {
   KvCache c;
@@ -71,7 +79,7 @@ struct AttnCfg {
   static constexpr int ROW = D * BITS / 8;                     // bytes of a cache row
   static constexpr int NG = BITS == 16 ? 1 : D / GS;           // quantization groups of a row
   static constexpr int TOK = ROW <= (BITS == 16 ? 128 : 96) ? 32 : 16;              // tokens per tile
-  static constexpr int PITCH = BITS == 16 && ROW % 128 ? ROW + 16 : ROW;
+  static constexpr int PITCH = ROW % 128 && ROW % 32 == 0 && ROW > 64 ? ROW + 16 : ROW;
   static constexpr int CH = ROW / 16;                          // 16-byte chunks per row
   static constexpr int STAGE = 2 * TOK * (PITCH + (BITS == 16 ? 0 : 8 * NG));   // bytes: keys, values, their scales
   static constexpr int ROOM8 = 13900, ROOM6 = 18500;           // bytes a warp of eight, of six
@@ -84,14 +92,13 @@ struct AttnCfg {
   static constexpr int RPG = TOK / RG;
   static_assert(STAGES >= 2 && STAGE % 16 == 0 && CH * RG <= 32 && RPG % 2 == 0, "a tile's copies");
 
-  // Row r's 16-byte chunks are stored at chunk ^ swz(r), so that the rows that
-  // one read instruction touches lie on different banks: eight rows of 128
-  // (or 256) bytes for ldmatrix; for codes the four rows whose 32 bytes a
-  // half-warp reads. 192-byte rows are padded instead.
+  // Row r's 16-byte chunks are stored at chunk ^ swz(r), or rows have an odd
+  // number of chunks, so that the eight rows that one matrix load touches lie
+  // on different banks.
   static __device__ __forceinline__ int swz(int r) {
-    if constexpr (BITS == 16) return ROW % 128 == 0 ? (r & 7) : 0;
-    else if constexpr (ROW == 128) return 2 * (((r & 7) + ((r >> 2) & 1)) & 3);
-    else if constexpr (ROW == 64) return 2 * ((r >> 1) & 1);
+    if constexpr (ROW % 128 == 0) return r & 7;
+    else if constexpr (ROW == 64) return (r >> 1) & 3;
+    else if constexpr (ROW == 32) return (r >> 2) & 1;
     else return 0;
   }
 };
@@ -117,6 +124,13 @@ __device__ __forceinline__ void ldsm4(unsigned (&r)[4], unsigned addr) {
   else
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldsm2(unsigned (&r)[2], unsigned addr) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ unsigned transpose8x8(unsigned x) {
   unsigned y;
@@ -241,7 +255,9 @@ struct AttnCursor {
 
 // D: head dimension; BITS: of the cache (16: rows of T); GS: quantization
 // group (of codes); NQ: query heads per pass, 4 or 8.
-template <typename T, int D, int BITS, int GS, int NQ>
+// SEG: a CTA per segment, its tiles split over the CTA's warps and joined in
+// shared memory; else the list of all segments' tiles split over all warps.
+template <typename T, int D, int BITS, int GS, int NQ, bool SEG>
 __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS) attn_kernel(AttnArgs a) {
   using Cfg = AttnCfg<D, BITS, GS, NQ>;
   using M = typename std::conditional<BITS == 16, T, __half>::type;   // type of the products' operands
@@ -255,7 +271,7 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
   constexpr float MID = (float)(1 << (BITS - 1));  // codes: value = scale (code - MID) + (bias + MID scale)
   constexpr unsigned ALL = TOK == 32 ? 0xffffffffu : 0xffffu;
   extern __shared__ __align__(128) unsigned char asm_raw[];
-  __shared__ int P[ATT_MAXB + 1];
+  __shared__ int P[SEG ? 1 : ATT_MAXB + 1];
   __shared__ int red[WARPS];
   __shared__ unsigned tmask[WARPS][ST];            // a stage's visible tokens
   __shared__ __align__(16) long long roff[WARPS][TOK];   // byte offsets of the rows of the tile being copied
@@ -263,37 +279,60 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
   grid_dep_wait();                                 // the cache's and the query's producers
   grid_dep_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  attn_prefix<WARPS>(a, TOK, P, red);
   const int QB = (a.G + NQ - 1) / NQ;              // passes over a key head's query heads
-
-  // sequences with nothing to see: zeros
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    if (P[b + 1] != P[b]) continue;
-    for (int j = threadIdx.x; j < a.c.heads * a.G * D; j += 32 * WARPS)
-      static_cast<T*>(a.out)[(long long)b * a.ob + (long long)(j / D) * a.oh + j % D] = Cvt<T>::t(0.0f);
+  int W = 0, w = 0, count = 0;
+  long long tiles = 0, t0 = 0;
+  AttnCursor look;
+  if constexpr (SEG) {
+    const int seg = blockIdx.x, HB = a.c.heads * QB, h = seg % HB;
+    look.b = seg / HB;
+    look.kvh = h / QB;
+    look.qb = h - look.kvh * QB;
+    long long lo, hi;
+    kv_visible(a.len[look.b], a.start ? a.start[look.b] : 0, a.max_pages, a.c.page_size, lo, hi);
+    look.lo = (unsigned)lo;
+    look.hi = (unsigned)hi;
+    look.nt = (int)kv_tiles(lo, hi, TOK);
+    if (look.nt == 0) {                            // nothing to see: zeros
+      for (int j = threadIdx.x; j < NQ * D; j += 32 * WARPS)
+        if (look.qb * NQ + j / D < a.G)
+          static_cast<T*>(a.out)[(long long)look.b * a.ob + (long long)(look.kvh * a.G + look.qb * NQ + j / D) * a.oh + j % D] =
+              Cvt<T>::t(0.0f);
+      return;
+    }
+    look.i = (int)((long long)look.nt * warp / WARPS);
+    count = (int)((long long)look.nt * (warp + 1) / WARPS) - look.i;
+  } else {
+    attn_prefix<WARPS>(a, TOK, P, red);
+    // sequences with nothing to see: zeros
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      if (P[b + 1] != P[b]) continue;
+      for (int j = threadIdx.x; j < a.c.heads * a.G * D; j += 32 * WARPS)
+        static_cast<T*>(a.out)[(long long)b * a.ob + (long long)(j / D) * a.oh + j % D] = Cvt<T>::t(0.0f);
+    }
+    tiles = (long long)P[a.B] * (a.c.heads * QB);
+    W = split_workers(tiles, gridDim.x * WARPS);
+    w = warp * gridDim.x + blockIdx.x;             // few tiles spread over the SMs first
+    if (w >= W) {
+      if (lane == 0) a.cut[w] = make_int4(0, 0, 0, 0);
+      return;
+    }
+    t0 = split_begin(tiles, W, w);
+    count = (int)(split_begin(tiles, W, w + 1) - t0);
+    look.seek(a, P, QB, t0);
   }
-
-  const long long tiles = (long long)P[a.B] * (a.c.heads * QB);
-  const int W = split_workers(tiles, gridDim.x * WARPS);
-  const int w = warp * gridDim.x + blockIdx.x;     // few tiles spread over the SMs first
-  if (w >= W) {
-    if (lane == 0) a.cut[w] = make_int4(0, 0, 0, 0);
-    return;
-  }
-  const long long t0 = split_begin(tiles, W, w);
-  const int count = (int)(split_begin(tiles, W, w + 1) - t0);
 
   unsigned char* my = asm_raw + warp * (ST * STAGE);
   const unsigned my_s = smem_u32(my);
 
   // ---- the copies' side: the page of each lane's token is looked up one tile ahead of its copy ----
-  AttnCursor look;
-  look.seek(a, P, QB, t0);
   int looked = 0;                                  // tiles looked up so far
   int lk_page = 0, lk_slot = 0;
   bool lk_in = false;
   auto lookup = [&]() {
-    if (looked++ > 0 && ++look.i == look.nt) look.next_segment(a, P, QB);
+    if (looked++ > 0 && ++look.i == look.nt) {
+      if constexpr (!SEG) look.next_segment(a, P, QB);
+    }
     const unsigned pos = look.lo + look.i * TOK + lane;
     lk_in = lane < TOK && pos < look.hi;
     if (lk_in) {                                   // inside the table: hi is cut to its width
@@ -370,7 +409,7 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
       for (int e = 0; e < 4; ++e) {
         int d;
         if (!CODES) d = 16 * s + 2 * t + (e & 1) + 8 * (e >> 1);
-        else if (BITS == 8) d = 32 * (s >> 1) + 8 * t + 4 * (s & 1) + e;
+        else if (BITS == 8) d = 16 * s + 4 * t + e;
         else d = 32 * (s >> 1) + 8 * t + 2 * (s & 1) + (e >> 1) + 4 * (e & 1);   // a pair is (i, i + 4)
         x[s][e] = have ? Cvt<T>::f(q[d]) : 0.0f;
       }
@@ -451,34 +490,32 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
           mma16816<M>(acc[0], r, qf[ks][0], qf[ks][1]);
         }
       } else {
-        const unsigned char* r0 = pk + (mb * 16 + g) * PITCH;                // rows g and g + 8: one swizzle
-        const unsigned char* r1 = r0 + 8 * PITCH;
-        const int x = Cfg::swz(g);
+        const unsigned base = sk + (mb * 16 + (lane & 15)) * PITCH;
+        const int x = Cfg::swz(lane & 15), hi = lane >> 4;
 #pragma unroll
         for (int blk = 0; blk < D / 32; ++blk) {
           unsigned f[2][4];
           if constexpr (BITS == 8) {
-            const int at = ((2 * blk) ^ x) * 16 + t * 8;                     // 8 codes
-            const uint2 u = *reinterpret_cast<const uint2*>(r0 + at);
-            const uint2 v = *reinterpret_cast<const uint2*>(r1 + at);
+            // a chunk is 16 codes, one k-step: this lane gets codes 4t .. 4t + 3 of rows g and g + 8
+            unsigned r[4];
+            ldsm4<false>(r, base + (((2 * blk + hi) ^ x) << 4));
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const unsigned xw = h ? u.y : u.x, yw = h ? v.y : v.x;
-              f[h][0] = half_codes<BITS>(__byte_perm(xw, 0x64646464u, 0x4140));
-              f[h][1] = half_codes<BITS>(__byte_perm(yw, 0x64646464u, 0x4140));
-              f[h][2] = half_codes<BITS>(__byte_perm(xw, 0x64646464u, 0x4342));
-              f[h][3] = half_codes<BITS>(__byte_perm(yw, 0x64646464u, 0x4342));
+              f[h][0] = half_codes<BITS>(__byte_perm(r[2 * h], 0x64646464u, 0x4140));
+              f[h][1] = half_codes<BITS>(__byte_perm(r[2 * h + 1], 0x64646464u, 0x4140));
+              f[h][2] = half_codes<BITS>(__byte_perm(r[2 * h], 0x64646464u, 0x4342));
+              f[h][3] = half_codes<BITS>(__byte_perm(r[2 * h + 1], 0x64646464u, 0x4342));
             }
           } else {
-            const int at = (blk ^ x) * 16 + t * 4;                           // 8 codes
-            const unsigned u = *reinterpret_cast<const unsigned*>(r0 + at);
-            const unsigned v = *reinterpret_cast<const unsigned*>(r1 + at);
+            // a chunk is 32 codes, two k-steps: codes 8t .. 8t + 7, taken in pairs (i, i + 4)
+            unsigned r[2];
+            ldsm2<false>(r, base + ((blk ^ x) << 4));
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              f[h][0] = half_codes<BITS>(((u >> (8 * h)) & 0x000f000fu) | 0x64006400u);
-              f[h][1] = half_codes<BITS>(((v >> (8 * h)) & 0x000f000fu) | 0x64006400u);
-              f[h][2] = half_codes<BITS>(((u >> (8 * h + 4)) & 0x000f000fu) | 0x64006400u);
-              f[h][3] = half_codes<BITS>(((v >> (8 * h + 4)) & 0x000f000fu) | 0x64006400u);
+              f[h][0] = half_codes<BITS>(((r[0] >> (8 * h)) & 0x000f000fu) | 0x64006400u);
+              f[h][1] = half_codes<BITS>(((r[1] >> (8 * h)) & 0x000f000fu) | 0x64006400u);
+              f[h][2] = half_codes<BITS>(((r[0] >> (8 * h + 4)) & 0x000f000fu) | 0x64006400u);
+              f[h][3] = half_codes<BITS>(((r[1] >> (8 * h + 4)) & 0x000f000fu) | 0x64006400u);
             }
           }
 #pragma unroll
@@ -562,7 +599,7 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
           for (int n = 0; n < NG; ++n) sb[n] = vsb[(mb * 16 + 8 * r + g) * NG + n];
 #pragma unroll
         for (int u = 0; u < QN; ++u) {
-          const float p = exp2f(s[mb][r][u] - base[u]);
+          const float p = ex2_approx(s[mb][r][u] - base[u]);
           l[u] += p;
           if constexpr (CODES) {
 #pragma unroll
@@ -586,46 +623,36 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
           for (int u = 0; u < QN; ++u) mma16816<M>(o[u][ks], r, pf[0][u][0], pf[0][u][1]);
         }
       } else {
-        // a group of GS dims: this lane's GS / 8 consecutive ones (from g GS / 8) for tokens 2t, 2t+1, +8, +9
-        const unsigned char* r0 = pv + (mb * 16 + 2 * t) * PITCH;
-        constexpr int LB = GS * BITS / 64;         // a lane's bytes of the group: 8, 4 or 2
-        const int xa = Cfg::swz(2 * t), xb = Cfg::swz(2 * t + 1);
+        // transposed loads of code pairs (8 bits) or quadruples (4): a register holds this lane's codes of token 2t in
+        // its low half and of 2t + 1 in its high half
+        const unsigned vb = sv + (mb * 16 + (lane & 15)) * PITCH;
+        const int x = Cfg::swz(lane & 15), hi = lane >> 4;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-          const int at = n * (GS * BITS / 8) + g * LB;
-          const int ca = (((at >> 4) ^ xa) << 4) + (at & 15), cb = (((at >> 4) ^ xb) << 4) + (at & 15) + PITCH;
           unsigned f[GS / 16][4];                  // [row block][a0..a3]
 #pragma unroll
-          for (int hv = 0; hv < 2; ++hv) {         // tokens 2t, 2t+1, then 2t+8, 2t+9
-            const unsigned char* ra = r0 + 8 * hv * PITCH + ca;
-            const unsigned char* rb = r0 + 8 * hv * PITCH + cb;
-            unsigned wa[2], wb[2];
-            if constexpr (LB == 8) {
-              const uint2 p = *reinterpret_cast<const uint2*>(ra), q = *reinterpret_cast<const uint2*>(rb);
-              wa[0] = p.x, wa[1] = p.y, wb[0] = q.x, wb[1] = q.y;
-            } else if constexpr (LB == 4) {
-              wa[0] = *reinterpret_cast<const unsigned*>(ra), wb[0] = *reinterpret_cast<const unsigned*>(rb);
-            } else {
-              wa[0] = *reinterpret_cast<const unsigned short*>(ra), wb[0] = *reinterpret_cast<const unsigned short*>(rb);
-            }
+          for (int wd = 0; wd < GS / 32; ++wd) {   // 32 dims: two row blocks
+            const int blk = n * (GS / 32) + wd;
             if constexpr (BITS == 8) {
+              unsigned r[4];                       // chunk 2 blk: tokens 0-7, 8-15; chunk 2 blk + 1
+              ldsm4<true>(r, vb + (((2 * blk + hi) ^ x) << 4));
 #pragma unroll
-              for (int wd = 0; wd < GS / 32; ++wd) {
-                const unsigned lo = __byte_perm(wa[wd], wb[wd], 0x5140), hi = __byte_perm(wa[wd], wb[wd], 0x7362);
-                f[2 * wd][2 * hv] = half_codes<BITS>(__byte_perm(lo, 0x64646464u, 0x4140));
-                f[2 * wd][2 * hv + 1] = half_codes<BITS>(__byte_perm(lo, 0x64646464u, 0x4342));
-                f[2 * wd + 1][2 * hv] = half_codes<BITS>(__byte_perm(hi, 0x64646464u, 0x4140));
-                f[2 * wd + 1][2 * hv + 1] = half_codes<BITS>(__byte_perm(hi, 0x64646464u, 0x4342));
-              }
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int hv = 0; hv < 2; ++hv) {
+                  f[2 * wd + h][2 * hv] = half_codes<BITS>(__byte_perm(r[2 * h + hv], 0x64646464u, 0x4240));
+                  f[2 * wd + h][2 * hv + 1] = half_codes<BITS>(__byte_perm(r[2 * h + hv], 0x64646464u, 0x4341));
+                }
             } else {
+              unsigned r[2];                       // chunk blk: tokens 0-7, 8-15
+              ldsm2<true>(r, vb + ((blk ^ x) << 4));
 #pragma unroll
-              for (int wd = 0; wd < GS / 32; ++wd) {           // 16 bits: four codes of each token
-                const unsigned x = __byte_perm(wa[0], wb[0], wd ? 0x7632 : 0x5410);
-                f[2 * wd][2 * hv] = half_codes<BITS>((x & 0x000f000fu) | 0x64006400u);
-                f[2 * wd][2 * hv + 1] = half_codes<BITS>(((x >> 4) & 0x000f000fu) | 0x64006400u);
-                f[2 * wd + 1][2 * hv] = half_codes<BITS>(((x >> 8) & 0x000f000fu) | 0x64006400u);
-                f[2 * wd + 1][2 * hv + 1] = half_codes<BITS>(((x >> 12) & 0x000f000fu) | 0x64006400u);
-              }
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int hv = 0; hv < 2; ++hv) {
+                  f[2 * wd + h][2 * hv] = half_codes<BITS>(((r[hv] >> (8 * h)) & 0x000f000fu) | 0x64006400u);
+                  f[2 * wd + h][2 * hv + 1] = half_codes<BITS>(((r[hv] >> (8 * h + 4)) & 0x000f000fu) | 0x64006400u);
+                }
             }
           }
 #pragma unroll
@@ -637,49 +664,58 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
     }
   };
 
-  // the segment (or this warp's part of it) is done: to the output, or to the parts
-  auto end_segment = [&](bool first, bool last) {
-    const int qb = cur.qb, kvh = cur.kvh;
+  // element e of row block ks of this lane's part of O^T: which dimension, and its value for query head u
+  const auto out_dim = [&](int ks, int e) {
+    if constexpr (BITS == 8) return 16 * ks + 2 * g + e;
+    else if constexpr (BITS == 4) return 32 * (ks >> 1) + 4 * g + 2 * (ks & 1) + e;
+    else return 16 * ks + 8 * e + g;
+  };
+  const auto each_out = [&](int u, auto&& put) {
     const float back = CODES ? smax / PSCALE : 1.0f / PSCALE;
+    [[maybe_unused]] float bias[CODES ? NG : 1];
+    if constexpr (CODES)
+#pragma unroll
+      for (int n = 0; n < NG; ++n) bias[n] = rows_sum(ob[n][u]);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = (o[u][ks][2 * e] + o[u][ks][2 * e + 1]) * back;
+        if constexpr (CODES) v += bias[ks / (GS / 16)];
+        put(out_dim(ks, e), v);
+      }
+  };
+  // this warp's part: [NQ][D] sums, [NQ][2] maxima and sums of weights
+  auto put_parts = [&](float* po, float* ml) {
 #pragma unroll
     for (int u = 0; u < QN; ++u) {
       const int jq = NQ == 4 ? t : 2 * t + u;      // within the pass
-      const int j = qb * NQ + jq;
       const float lt = rows_sum(l[u]);
-      float bias[CODES ? NG : 1];
-      if constexpr (CODES)
-#pragma unroll
-        for (int n = 0; n < NG; ++n) bias[n] = rows_sum(ob[n][u]);
-      if (j >= a.G) continue;
-      const bool whole = first && last;
-      const float f = whole ? 1.0f / lt : 1.0f;
-      T* out = static_cast<T*>(a.out) + (long long)cur.b * a.ob + (long long)(kvh * a.G + j) * a.oh;
-      const long long slot = ((long long)w * 2 + (first ? 1 : 0)) * NQ + jq;
-      float* po = a.part_o + slot * D;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float v = (o[u][ks][2 * e] + o[u][ks][2 * e + 1]) * back;
-          int d;
-          if constexpr (CODES) {
-            constexpr int RB = GS / 16;            // row blocks per group
-            d = (ks / RB) * GS + g * (GS / 8) + 2 * (ks % RB) + e;
-            v += bias[ks / RB];
-          } else {
-            d = 16 * ks + 8 * e + g;
-          }
-          if (whole) out[d] = Cvt<T>::t(v * f);
-          else po[d] = v;
-        }
-      if (!whole && g == 0) {
-        a.part_ml[slot * 2] = m[u];
-        a.part_ml[slot * 2 + 1] = lt;
+      each_out(u, [&](int d, float v) { po[jq * D + d] = v; });
+      if (g == 0) {
+        ml[jq * 2] = m[u];
+        ml[jq * 2 + 1] = lt;
       }
     }
   };
+  // the segment (or this warp's part of it) is done: to the output, or to the parts
+  auto end_segment = [&](bool first, bool last) {
+    if (!(first && last)) {
+      const long long slot = ((long long)w * 2 + (first ? 1 : 0)) * NQ;
+      put_parts(a.part_o + slot * D, a.part_ml + slot * 2);
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < QN; ++u) {
+      const int j = cur.qb * NQ + (NQ == 4 ? t : 2 * t + u);
+      const float f = 1.0f / rows_sum(l[u]);
+      T* out = static_cast<T*>(a.out) + (long long)cur.b * a.ob + (long long)(cur.kvh * a.G + j) * a.oh;
+      const bool mine = j < a.G;
+      each_out(u, [&](int d, float v) { if (mine) out[d] = Cvt<T>::t(v * f); });
+    }
+  };
 
-  lookup();
+  if (!SEG || count > 0) lookup();
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s) {
     if (s < count) {
@@ -702,79 +738,140 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
     cp_commit();
     compute(stage);
     stage = stage + 1 == ST ? 0 : stage + 1;
-    const bool seg_end = cur.i + 1 == cur.nt;
-    if (seg_end || n + 1 == count) end_segment(seg_first == 0, seg_end);
-    if (n + 1 < count) {
-      ++cur.i;
-      if (seg_end) {
-        cur.next_segment(a, P, QB);
-        seg_first = 0;
-        begin_segment();
+    if constexpr (!SEG) {
+      const bool seg_end = cur.i + 1 == cur.nt;
+      if (seg_end || n + 1 == count) end_segment(seg_first == 0, seg_end);
+      if (n + 1 < count) {
+        ++cur.i;
+        if (seg_end) {
+          cur.next_segment(a, P, QB);
+          seg_first = 0;
+          begin_segment();
+        }
+      } else if (lane == 0) {
+        const bool cuts = seg_first == 0 && !seg_end;
+        const long long end = t0 + n - cur.i + cur.nt;         // the tile behind the segment
+        a.cut[w] = make_int4(cuts ? split_owner(tiles, W, end - 1) - w + 1 : 0, cur.b, cur.kvh, cur.qb);
       }
-    } else if (lane == 0) {
-      const bool cuts = seg_first == 0 && !seg_end;
-      const long long end = t0 + n - cur.i + cur.nt;           // the tile behind the segment
-      a.cut[w] = make_int4(cuts ? split_owner(tiles, W, end - 1) - w + 1 : 0, cur.b, cur.kvh, cur.qb);
+    }
+  }
+  if constexpr (SEG) {
+    // the warps' parts meet in shared memory, where their tiles were
+    float* po = reinterpret_cast<float*>(asm_raw);             // [WARPS][NQ][D]
+    float* ml = po + WARPS * NQ * D;                           // [WARPS][NQ][2]
+    static_assert(WARPS * NQ * (D + 2) * 4 <= Cfg::SMEM, "the parts fit where the tiles were");
+    __syncthreads();
+    put_parts(po + (size_t)warp * NQ * D, ml + warp * NQ * 2);
+    __syncthreads();
+    for (int j = threadIdx.x; j < NQ * D; j += 32 * WARPS) {
+      const int jq = j / D, d = j - jq * D, hq = cur.qb * NQ + jq;
+      if (hq >= a.G) break;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < WARPS; ++i) mx = fmaxf(mx, ml[(i * NQ + jq) * 2]);
+      const float base = mx == -INFINITY ? 0.0f : mx;
+      float l = 0.0f, v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < WARPS; ++i) {
+        const float f = exp2f(ml[(i * NQ + jq) * 2] - base);
+        l = fmaf(f, ml[(i * NQ + jq) * 2 + 1], l);
+        v = fmaf(f, po[(size_t)(i * NQ + jq) * D + d], v);
+      }
+      static_cast<T*>(a.out)[(long long)cur.b * a.ob + (long long)(cur.kvh * a.G + hq) * a.oh + d] = Cvt<T>::t(v / l);
     }
   }
 }
 
-// Joins the segments that a border between two warps' shares cuts: CTA (w, j)
-// sums, for query head j of the pass, the parts of the segment that warp w
-// began, in an order that depends on nothing but the lengths.
+// Joins the segments that a border between two warps' shares cuts, for query
+// head blockIdx.y of the pass: CTA x looks after eight warps of the main
+// kernel. The parts of a segment that one of them began are summed by one warp
+// here, or where there are many by the CTA; the order of the sums depends on
+// nothing but the lengths.
+constexpr int ATT_JOIN_FEW = 16;                   // parts that one warp joins
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(ATT_JOIN_NT) attn_join_kernel(AttnArgs a) {
-  constexpr int NTH = ATT_JOIN_NT, COLS = D / 4, GR = NTH / COLS;   // GR groups of parts x COLS columns of four
-  __shared__ float fred[NTH / 32];
+__global__ void __launch_bounds__(ATT_JOIN_NT) attn_join_kernel(AttnArgs a, int W) {
+  constexpr int NTH = ATT_JOIN_NT, NW = NTH / 32, COLS = D / 4, GR = NTH / COLS;   // GR groups of parts x COLS columns of four
+  __shared__ int4 cuts[NW];
+  __shared__ float fred[NW];
   __shared__ __align__(16) float osum[GR][D];
   __shared__ float lsum[GR];
   grid_dep_wait();
   grid_dep_launch();
-  const int w = blockIdx.x, jq = blockIdx.y;
-  const int4 cut = a.cut[w];
-  const int parts = cut.x, j = cut.w * NQ + jq;
-  if (parts == 0 || j >= a.G) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // part 0 is the warp's own (it began the segment), the others are what later warps continued
-  auto slot = [&](int i) { return ((long long)(w + i) * 2 + (i == 0 ? 1 : 0)) * NQ + jq; };
-  float mx = -INFINITY;
-  for (int i = tid; i < parts; i += NTH) mx = fmaxf(mx, a.part_ml[slot(i) * 2]);
-  mx = warp_reduce(mx, [](float x, float y) { return fmaxf(x, y); });
-  if (lane == 0) fred[warp] = mx;
-  __syncthreads();
-  mx = fred[0];
-#pragma unroll
-  for (int i = 1; i < NTH / 32; ++i) mx = fmaxf(mx, fred[i]);
-  const float base = mx == -INFINITY ? 0.0f : mx;
-  const int col = tid % COLS, gr = tid / COLS;
-  if (gr < GR) {
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.0f;
-#pragma unroll 4
-    for (int i = gr; i < parts; i += GR) {
-      const long long s = slot(i);
-      const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[s];
-      const float4 v = reinterpret_cast<const float4*>(a.part_o + s * D)[col];
-      const float f = exp2f(ml.x - base);
-      l = fmaf(f, ml.y, l);
-      o.x = fmaf(f, v.x, o.x);
-      o.y = fmaf(f, v.y, o.y);
-      o.z = fmaf(f, v.z, o.z);
-      o.w = fmaf(f, v.w, o.w);
-    }
-    reinterpret_cast<float4*>(osum[gr])[col] = o;
-    if (col == 0) lsum[gr] = l;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, jq = blockIdx.y;
+  if (tid < NW) {
+    const int w = blockIdx.x * NW + tid;
+    cuts[tid] = w < W ? a.cut[w] : make_int4(0, 0, 0, 0);
   }
   __syncthreads();
-  float l = 0.0f;
+  // part 0 is the beginning warp's own, the others are what later warps continued
+  auto slot = [&](int w, int i) { return ((long long)(w + i) * 2 + (i == 0 ? 1 : 0)) * NQ + jq; };
+  auto place = [&](const int4& c) {
+    return static_cast<T*>(a.out) + (long long)c.y * a.ob + (long long)(c.z * a.G + c.w * NQ + jq) * a.oh;
+  };
+  {
+    const int4 c = cuts[warp];
+    const int w = blockIdx.x * NW + warp;
+    if (c.x > 0 && c.x <= ATT_JOIN_FEW && c.w * NQ + jq < a.G) {
+      const float2 ml = lane < c.x ? reinterpret_cast<const float2*>(a.part_ml)[slot(w, lane)] : make_float2(-INFINITY, 0.0f);
+      const float mx = warp_reduce(ml.x, [](float x, float y) { return fmaxf(x, y); });
+      const float f = exp2f(ml.x - (mx == -INFINITY ? 0.0f : mx));
+      const float l = warp_reduce(f * ml.y, [](float x, float y) { return x + y; });
+      T* out = place(c);
+      constexpr int PER = D / 32;                  // elements a lane: lane, lane + 32, ...
+      float v[PER];
 #pragma unroll
-  for (int i = 0; i < GR; ++i) l += lsum[i];
-  T* out = static_cast<T*>(a.out) + (long long)cut.y * a.ob + (long long)(cut.z * a.G + j) * a.oh;
-  if (tid < D) {
-    float v = 0.0f;
+      for (int e = 0; e < PER; ++e) v[e] = 0.0f;
+#pragma unroll 4
+      for (int i = 0; i < c.x; ++i) {
+        const float fi = __shfl_sync(FULL, f, i);
+        const float* p = a.part_o + slot(w, i) * D + lane;
 #pragma unroll
-    for (int i = 0; i < GR; ++i) v += osum[i][tid];
-    out[tid] = Cvt<T>::t(v / l);
+        for (int e = 0; e < PER; ++e) v[e] = fmaf(fi, p[32 * e], v[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < PER; ++e) out[lane + 32 * e] = Cvt<T>::t(v[e] / l);
+    }
+  }
+  for (int item = 0; item < NW; ++item) {
+    const int4 c = cuts[item];
+    const int parts = c.x, w = blockIdx.x * NW + item;
+    if (parts <= ATT_JOIN_FEW || c.w * NQ + jq >= a.G) continue;       // the same for the whole CTA
+    float mx = -INFINITY;
+    for (int i = tid; i < parts; i += NTH) mx = fmaxf(mx, a.part_ml[slot(w, i) * 2]);
+    mx = warp_reduce(mx, [](float x, float y) { return fmaxf(x, y); });
+    if (lane == 0) fred[warp] = mx;
+    __syncthreads();
+    mx = fred[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) mx = fmaxf(mx, fred[i]);
+    const float base = mx == -INFINITY ? 0.0f : mx;
+    const int col = tid % COLS, gr = tid / COLS;
+    if (gr < GR) {
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.0f;
+#pragma unroll 8
+      for (int i = gr; i < parts; i += GR) {
+        const long long s = slot(w, i);
+        const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[s];
+        const float4 v = reinterpret_cast<const float4*>(a.part_o + s * D)[col];
+        const float f = exp2f(ml.x - base);
+        l = fmaf(f, ml.y, l);
+        o.x = fmaf(f, v.x, o.x);
+        o.y = fmaf(f, v.y, o.y);
+        o.z = fmaf(f, v.z, o.z);
+        o.w = fmaf(f, v.w, o.w);
+      }
+      reinterpret_cast<float4*>(osum[gr])[col] = o;
+      if (col == 0) lsum[gr] = l;
+    }
+    __syncthreads();
+    if (tid < D) {
+      float l = 0.0f, v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < GR; ++i) l += lsum[i], v += osum[i][tid];
+      place(c)[tid] = Cvt<T>::t(v / l);
+    }
+    __syncthreads();
   }
 }
 

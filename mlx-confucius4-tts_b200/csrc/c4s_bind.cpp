@@ -200,6 +200,43 @@ PyObject* kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// (ctx, device, cache, cache's device, page_table, pos, tok_off, total, c4s_dtype or -1) -> (k, v), one allocation
+PyObject* kv_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args a{args, n};
+    c4s_ctx* ctx = static_cast<c4s_ctx*>(a.pointer("context"));
+    const int dev = (int)a.integer("device");
+    const c4s_kv_cache* c = static_cast<const c4s_kv_cache*>(a.pointer("cache"));
+    const long long cdev = a.integer("cache device");
+    const Tensor &table = a.tensor("page_table"), &pos = a.tensor("pos");
+    const Tensor* off = a.maybe("tok_off");
+    const int64_t total = a.integer("total");
+    const int kind = (int)a.integer("dtype");
+    if (total < 0) value_error("total must not be negative");
+    if (cdev != dev) value_error("the cache is not on the context's device");
+    on(dev, &table, "page_table");
+    on(dev, &pos, "pos");
+    on(dev, off, "tok_off");
+    const at::ScalarType type = kind == C4S_FP32 ? at::kFloat
+                                : kind == C4S_FP16 || (kind < 0 && c->bits == 16 && c->dtype == C4S_FP16) ? at::kHalf
+                                                                                                           : at::kBFloat16;
+    const Tensor both = at::empty({2, total, c->kv_heads, c->head_dim}, pos.options().dtype(type));
+    const Tensor k = both.select(0, 0), v = both.select(0, 1);
+    const KvCall r = kv_ok(*c, table, k, v, pos, off, false);
+    const int rc = c4s_kv_read(ctx, c, table.const_data_ptr<int32_t>(), table.stride(0),
+                               int32_of(table.size(1), "the page table's width"), r.B, k.data_ptr(), v.data_ptr(), r.kind,
+                               k.stride(0), k.stride(1), r.T, off ? off->const_data_ptr<int64_t>() : nullptr,
+                               pos.const_data_ptr<int32_t>(), stream_of(dev));
+    if (rc) c_error(ctx, rc, "c4s_kv_read");
+    PyObject* pk = THPVariable_Wrap(k);
+    PyObject* pv = THPVariable_Wrap(v);
+    PyObject* out = pk && pv ? PyTuple_Pack(2, pk, pv) : nullptr;
+    Py_XDECREF(pk);
+    Py_XDECREF(pv);
+    return out;
+  });
+}
+
 // (cache, page_table, k, v, pos, tok_off, write): the checks alone -> (B, T, type)
 PyObject* check_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -269,7 +306,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!work) {
       const int64_t bytes = c4s_attention_workspace(ctx, r.B, r.heads, c->head_dim);
       if (bytes < 0) c_error(ctx, (int)bytes, "c4s_attention_workspace");
-      scratch = at::zeros({bytes}, q.options().dtype(at::kByte));
+      scratch = at::empty({bytes}, q.options().dtype(at::kByte));
       work = &scratch;
     }
     const int rc = c4s_paged_attention(
@@ -419,6 +456,7 @@ template <typename F> PyCFunction fast(F f) { return reinterpret_cast<PyCFunctio
 
 PyMethodDef methods[] = {
     {"kv", fast(kv), METH_FASTCALL, nullptr},
+    {"kv_read", fast(kv_read), METH_FASTCALL, nullptr},
     {"check_kv", fast(check_kv), METH_FASTCALL, nullptr},
     {"paged_attention", fast(paged_attention), METH_FASTCALL, nullptr},
     {"check_attention", fast(check_attention), METH_FASTCALL, nullptr},

@@ -131,13 +131,16 @@ template <typename TO> KvKernel read_kernel(int bits, int cache_dtype) {
 }
 
 using AttnKernel = void (*)(c4s::AttnArgs);
+using JoinKernel = void (*)(c4s::AttnArgs, int);
 struct AttnPick {
-  AttnKernel main = nullptr, join = nullptr;
+  AttnKernel main = nullptr, seg = nullptr;
+  JoinKernel join = nullptr;
   int smem = 0, tok = 0, warps = 0;
 };
 template <typename T, int D, int BITS, int GS, int NQ> AttnPick attn_pick() {
   using Cfg = c4s::AttnCfg<D, BITS, GS, NQ>;
-  return {c4s::attn_kernel<T, D, BITS, GS, NQ>, c4s::attn_join_kernel<T, D, NQ>, Cfg::SMEM, Cfg::TOK, Cfg::WARPS};
+  return {c4s::attn_kernel<T, D, BITS, GS, NQ, false>, c4s::attn_kernel<T, D, BITS, GS, NQ, true>,
+          c4s::attn_join_kernel<T, D, NQ>, Cfg::SMEM, Cfg::TOK, Cfg::WARPS};
 }
 template <typename T, int D, int NQ> AttnPick attn_pick_rows(int bits, int group) {
   if (bits == 16) return attn_pick<T, D, 16, 32, NQ>();
@@ -334,8 +337,6 @@ int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* 
                                     : attn_pick_dim<__nv_bfloat16, 8>(cache->head_dim, cache->bits, cache->group))
                          : (NQ == 4 ? attn_pick_dim<__half, 4>(cache->head_dim, cache->bits, cache->group)
                                     : attn_pick_dim<__half, 8>(cache->head_dim, cache->bits, cache->group));
-  cudaError_t e = cudaFuncSetAttribute(k.main, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
-  if (e != cudaSuccess) return cuda_fail(ctx, e, "attention kernel attribute");
   const int ctas = ctx->num_sms * c4s::ATT_CTAS;
   const int64_t warps = (int64_t)ctas * k.warps;
   c4s::AttnArgs a;
@@ -356,8 +357,28 @@ int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* 
   // tiles that the page table can name: a launch's prefix sums of them stay inside 32 bits
   const long long cap = std::min<long long>((long long)max_pages * cache->page_size, 0x7fffffffLL);
   const long long cap_tiles = c4s::kv_tiles(0, cap, k.tok);
-  const int group = (int)std::min<long long>(c4s::ATT_MAXB, 0x7fffffffLL / cap_tiles);
   const int passes = (G + NQ - 1) / NQ;
+  // A CTA per segment (a sequence's pass over one key head) needs no prefix sums and no second kernel: better where
+  // its warps have few tiles each, or no more than the tail of many such CTAs costs, by the lengths that the page
+  // table can name. Measured, us, CTA per segment / list over all warps: 20 heads of 64, one sequence of 700 5.9 / 7.7,
+  // 256 of up to 1500 156 / 172, 16 of up to 4000 38 / 43, 4 of up to 4000 21 / 16, 2 x 8 heads of 128 x 50001 501 /
+  // 72. Many segments shorter than a CTA's warps are better packed (64 x 20 of 59 tokens: 17 / 12.7).
+  const long long segs = (long long)B * cache->kv_heads * passes;
+  const long long per_warp = (cap_tiles + k.warps - 1) / k.warps;
+  const bool seg = (per_warp <= 8 || (per_warp <= 24 && segs * 5 >= (long long)ctas * 4)) &&
+                   (segs <= ctas || cap_tiles >= k.warps) && segs <= 0x7fffffffLL;
+  if (seg) {
+    a.B = B;
+    a.table = d_page_table;
+    a.q = d_q;
+    a.out = d_out;
+    a.len = d_len;
+    a.start = d_start;
+    cudaError_t e = cudaFuncSetAttribute(k.seg, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
+    if (e == cudaSuccess) e = launch(k.seg, dim3((unsigned)segs), 32 * k.warps, k.smem, stream, a);
+    return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "attention launch");
+  }
+  const int group = (int)std::min<long long>(c4s::ATT_MAXB, 0x7fffffffLL / cap_tiles);
   for (int b0 = 0; b0 < B; b0 += group) {
     a.B = std::min(group, B - b0);
     a.table = d_page_table + (int64_t)b0 * table_ld;
@@ -366,11 +387,12 @@ int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* 
     a.len = d_len + b0;
     a.start = d_start ? d_start + b0 : nullptr;
     // no more CTAs than there can be tiles for their first warps
-    const long long most = a.B * cap_tiles * cache->kv_heads * passes;
-    const int grid = (int)std::min<long long>(ctas, most);
-    e = launch(k.main, dim3((unsigned)grid), 32 * k.warps, k.smem, stream, a);
+    const int grid = (int)std::min<long long>(ctas, (long long)a.B * cache->kv_heads * passes * cap_tiles);
+    cudaError_t e = cudaFuncSetAttribute(k.main, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
+    if (e == cudaSuccess) e = launch(k.main, dim3((unsigned)grid), 32 * k.warps, k.smem, stream, a);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "attention launch");
-    e = launch(k.join, dim3((unsigned)(grid * k.warps), (unsigned)std::min(G, NQ)), c4s::ATT_JOIN_NT, 0, stream, a);
+    const int W = grid * k.warps, per = c4s::ATT_JOIN_NT / 32;
+    e = launch(k.join, dim3((unsigned)((W + per - 1) / per), (unsigned)std::min(G, NQ)), c4s::ATT_JOIN_NT, 0, stream, a, W);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "attention join launch");
   }
   return C4S_OK;

@@ -299,13 +299,17 @@ ATTENTION = [
 ]
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("bits,dtype,group", CACHES)
 @pytest.mark.parametrize("heads,shared,dim,page,lens,start", ATTENTION)
-def test_attention(ctx, c4s, bits, dtype, group, heads, shared, dim, page, lens, start):
+def test_attention(ctx, c4s, bits, dtype, group, heads, shared, dim, page, lens, start, wide):
+    """Both ways of splitting the work: a page table of the lengths' width, and one that could name far longer ones."""
     if dim % group:
         group = 32
     g = gen(heads * 100 + dim + bits)
     cache, table = filled(c4s, lens, heads, dim, page, dtype, bits, group, g, token_major=page % 2 == 0)
+    if wide:
+        table = torch.cat([table, torch.full((len(lens), 9000), -1, dtype=torch.int32, device=DEV)], 1)
     q = (torch.randn((len(lens), heads * shared, dim), generator=g, device=DEV) * 0.8).to(dtype)
     scale = 1 / math.sqrt(dim)
     out = ctx.paged_attention(q, cache, table, i32(lens), start=None if start is None else i32(start))
@@ -326,13 +330,14 @@ def test_attention_joins_one_long_sequence(ctx, c4s, bits, dtype):
         check_attention(ctx, c4s, q, cache, table, lens, None, 0.125, out)
 
 
-def test_attention_many_sequences(ctx, c4s):
+@pytest.mark.parametrize("wide", [0, 3000])
+def test_attention_many_sequences(ctx, c4s, wide):
     """More sequences than one launch takes, most of them short, pages shared between them."""
     g = gen(10)
     B, base = 1100, [200, 40, 0, 3]
     cache, t4 = filled(c4s, base, 2, 64, 16, BF, 16, 64, g)
     lens = [base[b % 4] for b in range(B)]
-    table = t4.repeat(B // 4, 1)
+    table = torch.cat([t4.repeat(B // 4, 1), torch.full((B, wide), -1, dtype=torch.int32, device=DEV)], 1)
     q = torch.randn((B, 2, 64), generator=g, device=DEV).to(BF)
     out = ctx.paged_attention(q, cache, table, i32(lens))
     check_attention(ctx, c4s, q, cache, table, lens, None, 0.125, out)
@@ -393,12 +398,14 @@ def test_attention_bad_pages(ctx, c4s):
     assert (out[1, 0].double() - p @ v[1][:, 0]).abs().max() < 0.02
 
 
-def test_attention_repeats_and_graphs(ctx, c4s):
+@pytest.mark.parametrize("wide", [0, 5000])
+def test_attention_repeats_and_graphs(ctx, c4s, wide):
     """The same call gives the same bits; two graphs with workspaces of their own, replayed on two streams while
     lengths grow in place, give what the eager calls give."""
     g = gen(14)
     lens = [400, 33, 0, 1200]
     cache, table = filled(c4s, [n + 8 for n in lens], 4, 64, 16, BF, 8, 64, g, nan=False)
+    table = torch.cat([table, torch.full((4, wide), -1, dtype=torch.int32, device=DEV)], 1)
     q = torch.randn((4, 4, 64), generator=g, device=DEV).to(BF)
     n = i32(lens)
     a = ctx.paged_attention(q, cache, table, n)
