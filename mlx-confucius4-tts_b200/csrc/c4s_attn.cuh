@@ -39,9 +39,9 @@
 //     into fp16's upper range, p scale by the largest scale seen so far.
 //
 // Measured on one B200 (graph, warm; GB/s of the bytes that cannot be done
-// without): 256 ragged sequences of up to 1500, 20 heads of 64, bf16 156 us
-// (6180), 2 x 50001 x 8 heads of 128, fp16 72 us (5730), 64 of up to 1600 in
-// 8-bit codes 43 us (3410), one of 700 5.9 us.
+// without): 256 ragged sequences of up to 1500, 20 heads of 64, bf16 148 us
+// (6500), 2 x 50001 x 8 heads of 128, fp16 72 us (5730), 64 of up to 1600 in
+// 8-bit codes 42 us (3550), one of 700 6.3 us.
 #pragma once
 
 namespace c4s {
@@ -58,6 +58,7 @@ struct AttnArgs {
   const void* q;                                   // [B, heads_q, D] by its strides (elements)
   long long qb, qh;
   int G;                                           // query heads per key head
+  bool q_pairs;                                    // q's rows start on 4 bytes
   const int* len;
   const int* start;                                // or null
   float scale;                                     // times log2(e)
@@ -116,21 +117,26 @@ __device__ __forceinline__ void cp8(unsigned dst, const void* src, bool ok) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// Matrix loads that may be moved among themselves, so that several are under
+// way at once: their place is fixed by `after` (a value made after the wait
+// for the tile) and by the products that use them, which stay in order.
 template <bool TRANS>
-__device__ __forceinline__ void ldsm4(unsigned (&r)[4], unsigned addr) {
+__device__ __forceinline__ void ldsm4(unsigned (&r)[4], unsigned addr, unsigned after) {
   if constexpr (TRANS)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+    asm("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4]; // %5"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr), "r"(after));
   else
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+    asm("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4]; // %5"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr), "r"(after));
 }
 template <bool TRANS>
-__device__ __forceinline__ void ldsm2(unsigned (&r)[2], unsigned addr) {
+__device__ __forceinline__ void ldsm2(unsigned (&r)[2], unsigned addr, unsigned after) {
   if constexpr (TRANS)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+    asm("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2]; // %3"
+        : "=r"(r[0]), "=r"(r[1]) : "r"(addr), "r"(after));
   else
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+    asm("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2]; // %3"
+        : "=r"(r[0]), "=r"(r[1]) : "r"(addr), "r"(after));
 }
 __device__ __forceinline__ unsigned transpose8x8(unsigned x) {
   unsigned y;
@@ -294,14 +300,15 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
     look.hi = (unsigned)hi;
     look.nt = (int)kv_tiles(lo, hi, TOK);
     if (look.nt == 0) {                            // nothing to see: zeros
-      for (int j = threadIdx.x; j < NQ * D; j += 32 * WARPS)
+      for (int j = threadIdx.x; j < NQ * D; j += blockDim.x)
         if (look.qb * NQ + j / D < a.G)
           static_cast<T*>(a.out)[(long long)look.b * a.ob + (long long)(look.kvh * a.G + look.qb * NQ + j / D) * a.oh + j % D] =
               Cvt<T>::t(0.0f);
       return;
     }
-    look.i = (int)((long long)look.nt * warp / WARPS);
-    count = (int)((long long)look.nt * (warp + 1) / WARPS) - look.i;
+    const int nw = blockDim.x >> 5;                // warps of the launch, at most WARPS
+    look.i = (int)((long long)look.nt * warp / nw);
+    count = (int)((long long)look.nt * (warp + 1) / nw) - look.i;
   } else {
     attn_prefix<WARPS>(a, TOK, P, red);
     // sequences with nothing to see: zeros
@@ -402,16 +409,40 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
     const int j = qb * NQ + col;
     const bool have = col >= 0 && j < a.G;
     const T* q = static_cast<const T*>(a.q) + (long long)cur.b * a.qb + (have ? (long long)(kvh * a.G + j) * a.qh : 0);
+    // All loads at once, and a column without a query reads its neighbour's: a branch around each would make the
+    // lane wait for one after the other.
+    unsigned pr[KS][2];
+    auto at = [&](int s, int h) {                  // elements d and d + 1 of the pair
+      return BITS == 4 ? 32 * (s >> 1) + 8 * t + 4 * (s & 1) + 2 * h : BITS == 8 ? 16 * s + 4 * t + 2 * h : 16 * s + 2 * t + 8 * h;
+    };
+    if (a.q_pairs) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) pr[s][h] = *reinterpret_cast<const unsigned*>(q + at(s, h));
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) pr[s][h] = pack2<T>(q[at(s, h)], q[at(s, h) + 1]);
+    }
     float x[KS][4];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        int d;
-        if (!CODES) d = 16 * s + 2 * t + (e & 1) + 8 * (e >> 1);
-        else if (BITS == 8) d = 16 * s + 4 * t + e;
-        else d = 32 * (s >> 1) + 8 * t + 2 * (s & 1) + (e >> 1) + 4 * (e & 1);   // a pair is (i, i + 4)
-        x[s][e] = have ? Cvt<T>::f(q[d]) : 0.0f;
+      for (int h = 0; h < 2; ++h) {
+        T v[2];
+        memcpy(v, &pr[s][h], 4);
+        const float v0 = have ? Cvt<T>::f(v[0]) : 0.0f, v1 = have ? Cvt<T>::f(v[1]) : 0.0f;
+        if constexpr (BITS == 4) {
+          // codes i and i + 1 of the lane's eight of a 32-block; in the products an element is paired with i + 4
+          const int i = 4 * (s & 1) + 2 * h;
+          x[(s & ~1) + ((i & 3) >> 1)][i >> 2] = v0;
+          x[(s & ~1) + ((i & 3) >> 1)][2 + (i >> 2)] = v1;
+        } else {
+          x[s][2 * h] = v0;
+          x[s][2 * h + 1] = v1;
+        }
       }
     float up = 1.0f, down = 1.0f;
     if constexpr (CODES) {
@@ -467,61 +498,68 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
   auto compute = [&](int stage) {
     const unsigned sk = my_s + stage * STAGE, sv = sk + TOK * PITCH;
     const unsigned char* pk = my + stage * STAGE;
-    const unsigned char* pv = pk + TOK * PITCH;
     const float2* ksb = reinterpret_cast<const float2*>(pk + 2 * TOK * PITCH);
     const float2* vsb = ksb + TOK * NG;
     const unsigned mask = tmask[warp][stage];
-    // scores of the tile: rows g and g + 8 of each 16-token block, the lane's query heads
-    float s[MB][2][QN];
+    unsigned now;                                  // the tile is there: no load of it before this
+    asm volatile("mov.u32 %0, %1;" : "=r"(now) : "r"(mask) : "memory");
+    // scores of the tile: rows g and g + 8 of each 16-token block, the lane's query heads; the blocks' chains of
+    // products take turns
+    float s[MB][2][QN], acc[MB][NG][4];
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      float acc[NG][4];
+    for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) acc[mb][n][e] = 0.0f;
+    {
+      const unsigned base = sk + (lane & 15) * PITCH;
+      const int x = Cfg::swz(lane & 15), hi = lane >> 4;
       if constexpr (!CODES) {
-        const unsigned base = sk + (mb * 16 + (lane & 15)) * PITCH;
-        const int x = Cfg::swz(lane & 15) ^ (lane >> 4);       // chunk 2 ks + (lane >> 4) of its row
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          unsigned r[4];
-          ldsm4<false>(r, base + (((2 * ks) ^ x) << 4));
-          mma16816<M>(acc[0], r, qf[ks][0], qf[ks][1]);
-        }
-      } else {
-        const unsigned base = sk + (mb * 16 + (lane & 15)) * PITCH;
-        const int x = Cfg::swz(lane & 15), hi = lane >> 4;
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int blk = 0; blk < D / 32; ++blk) {
-          unsigned f[2][4];
-          if constexpr (BITS == 8) {
-            // a chunk is 16 codes, one k-step: this lane gets codes 4t .. 4t + 3 of rows g and g + 8
+          for (int mb = 0; mb < MB; ++mb) {
             unsigned r[4];
-            ldsm4<false>(r, base + (((2 * blk + hi) ^ x) << 4));
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              f[h][0] = half_codes<BITS>(__byte_perm(r[2 * h], 0x64646464u, 0x4140));
-              f[h][1] = half_codes<BITS>(__byte_perm(r[2 * h + 1], 0x64646464u, 0x4140));
-              f[h][2] = half_codes<BITS>(__byte_perm(r[2 * h], 0x64646464u, 0x4342));
-              f[h][3] = half_codes<BITS>(__byte_perm(r[2 * h + 1], 0x64646464u, 0x4342));
-            }
-          } else {
-            // a chunk is 32 codes, two k-steps: codes 8t .. 8t + 7, taken in pairs (i, i + 4)
-            unsigned r[2];
-            ldsm2<false>(r, base + ((blk ^ x) << 4));
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              f[h][0] = half_codes<BITS>(((r[0] >> (8 * h)) & 0x000f000fu) | 0x64006400u);
-              f[h][1] = half_codes<BITS>(((r[1] >> (8 * h)) & 0x000f000fu) | 0x64006400u);
-              f[h][2] = half_codes<BITS>(((r[0] >> (8 * h + 4)) & 0x000f000fu) | 0x64006400u);
-              f[h][3] = half_codes<BITS>(((r[1] >> (8 * h + 4)) & 0x000f000fu) | 0x64006400u);
-            }
+            ldsm4<false>(r, base + mb * 16 * PITCH + (((2 * ks) ^ hi ^ x) << 4), now);
+            mma16816<M>(acc[mb][0], r, qf[ks][0], qf[ks][1]);
           }
+      } else {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) mma16816<M>(acc[32 * blk / GS], f[h], qf[2 * blk + h][0], qf[2 * blk + h][1]);
-        }
+        for (int blk = 0; blk < D / 32; ++blk)
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) {
+            unsigned f[2][4];
+            if constexpr (BITS == 8) {
+              // a chunk is 16 codes, one k-step: this lane gets codes 4t .. 4t + 3 of rows g and g + 8
+              unsigned r[4];
+              ldsm4<false>(r, base + mb * 16 * PITCH + (((2 * blk + hi) ^ x) << 4), now);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                f[h][0] = half_codes<BITS>(__byte_perm(r[2 * h], 0x64646464u, 0x4140));
+                f[h][1] = half_codes<BITS>(__byte_perm(r[2 * h + 1], 0x64646464u, 0x4140));
+                f[h][2] = half_codes<BITS>(__byte_perm(r[2 * h], 0x64646464u, 0x4342));
+                f[h][3] = half_codes<BITS>(__byte_perm(r[2 * h + 1], 0x64646464u, 0x4342));
+              }
+            } else {
+              // a chunk is 32 codes, two k-steps: codes 8t .. 8t + 7, taken in pairs (i, i + 4)
+              unsigned r[2];
+              ldsm2<false>(r, base + mb * 16 * PITCH + ((blk ^ x) << 4), now);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                f[h][0] = half_codes<BITS>(((r[0] >> (8 * h)) & 0x000f000fu) | 0x64006400u);
+                f[h][1] = half_codes<BITS>(((r[1] >> (8 * h)) & 0x000f000fu) | 0x64006400u);
+                f[h][2] = half_codes<BITS>(((r[0] >> (8 * h + 4)) & 0x000f000fu) | 0x64006400u);
+                f[h][3] = half_codes<BITS>(((r[1] >> (8 * h + 4)) & 0x000f000fu) | 0x64006400u);
+              }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) mma16816<M>(acc[mb][32 * blk / GS], f[h], qf[2 * blk + h][0], qf[2 * blk + h][1]);
+          }
       }
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int tok = mb * 16 + 8 * r + g;
@@ -537,9 +575,9 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
             v = 0.0f;
 #pragma unroll
             for (int n = 0; n < NG; ++n)
-              v = fmaf(sb[n].x, acc[n][2 * r + u], fmaf(fmaf(sb[n].x, MID, sb[n].y), qsum[n][u], v));
+              v = fmaf(sb[n].x, acc[mb][n][2 * r + u], fmaf(fmaf(sb[n].x, MID, sb[n].y), qsum[n][u], v));
           } else {
-            v = acc[0][2 * r + u];
+            v = acc[mb][0][2 * r + u];
           }
           s[mb][r][u] = seen ? v * qmul[u] : -INFINITY;
         }
@@ -618,7 +656,7 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           unsigned r[4];
-          ldsm4<true>(r, vb + (((2 * ks) ^ x) << 4));
+          ldsm4<true>(r, vb + (((2 * ks) ^ x) << 4), now);
 #pragma unroll
           for (int u = 0; u < QN; ++u) mma16816<M>(o[u][ks], r, pf[0][u][0], pf[0][u][1]);
         }
@@ -635,7 +673,7 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
             const int blk = n * (GS / 32) + wd;
             if constexpr (BITS == 8) {
               unsigned r[4];                       // chunk 2 blk: tokens 0-7, 8-15; chunk 2 blk + 1
-              ldsm4<true>(r, vb + (((2 * blk + hi) ^ x) << 4));
+              ldsm4<true>(r, vb + (((2 * blk + hi) ^ x) << 4), now);
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -645,7 +683,7 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
                 }
             } else {
               unsigned r[2];                       // chunk blk: tokens 0-7, 8-15
-              ldsm2<true>(r, vb + ((blk ^ x) << 4));
+              ldsm2<true>(r, vb + ((blk ^ x) << 4), now);
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -757,27 +795,28 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
   }
   if constexpr (SEG) {
     // the warps' parts meet in shared memory, where their tiles were
-    float* po = reinterpret_cast<float*>(asm_raw);             // [WARPS][NQ][D]
-    float* ml = po + WARPS * NQ * D;                           // [WARPS][NQ][2]
-    static_assert(WARPS * NQ * (D + 2) * 4 <= Cfg::SMEM, "the parts fit where the tiles were");
+    const int nw = blockDim.x >> 5;
+    float* po = reinterpret_cast<float*>(asm_raw);             // [nw][NQ][D]
+    float* ml = po + nw * NQ * D;                              // [nw][NQ][2]
+    static_assert(NQ * (D + 2) * 4 <= ST * STAGE, "a part fits where its warp's tiles were");
     __syncthreads();
-    put_parts(po + (size_t)warp * NQ * D, ml + warp * NQ * 2);
+    put_parts(po + warp * NQ * D, ml + warp * NQ * 2);
     __syncthreads();
-    for (int j = threadIdx.x; j < NQ * D; j += 32 * WARPS) {
-      const int jq = j / D, d = j - jq * D, hq = cur.qb * NQ + jq;
-      if (hq >= a.G) break;
+    const int live = min(NQ, a.G - cur.qb * NQ) * D;
+    for (int j = threadIdx.x; j < live; j += blockDim.x) {
+      const int jq = j / D, d = j - jq * D;
       float mx = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < WARPS; ++i) mx = fmaxf(mx, ml[(i * NQ + jq) * 2]);
+      for (int i = 0; i < nw; ++i) mx = fmaxf(mx, ml[(i * NQ + jq) * 2]);
       const float base = mx == -INFINITY ? 0.0f : mx;
       float l = 0.0f, v = 0.0f;
-#pragma unroll
-      for (int i = 0; i < WARPS; ++i) {
+#pragma unroll 4
+      for (int i = 0; i < nw; ++i) {
         const float f = exp2f(ml[(i * NQ + jq) * 2] - base);
         l = fmaf(f, ml[(i * NQ + jq) * 2 + 1], l);
-        v = fmaf(f, po[(size_t)(i * NQ + jq) * D + d], v);
+        v = fmaf(f, po[(i * NQ + jq) * D + d], v);
       }
-      static_cast<T*>(a.out)[(long long)cur.b * a.ob + (long long)(cur.kvh * a.G + hq) * a.oh + d] = Cvt<T>::t(v / l);
+      static_cast<T*>(a.out)[(long long)cur.b * a.ob + (long long)(cur.kvh * a.G + cur.qb * NQ + jq) * a.oh + d] =
+          Cvt<T>::t(v / l);
     }
   }
 }

@@ -347,6 +347,7 @@ int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* 
   a.qb = q_batch_stride;
   a.qh = q_head_stride;
   a.G = G;
+  a.q_pairs = ((uintptr_t)d_q & 3) == 0 && ((q_batch_stride | q_head_stride) & 1) == 0;
   a.scale = scale * 1.4426950408889634f;           // log2(e): the softmax works in powers of two
   a.ob = out_batch_stride;
   a.oh = out_head_stride;
@@ -361,12 +362,10 @@ int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* 
   // A CTA per segment (a sequence's pass over one key head) needs no prefix sums and no second kernel: better where
   // its warps have few tiles each, or no more than the tail of many such CTAs costs, by the lengths that the page
   // table can name. Measured, us, CTA per segment / list over all warps: 20 heads of 64, one sequence of 700 5.9 / 7.7,
-  // 256 of up to 1500 156 / 172, 16 of up to 4000 38 / 43, 4 of up to 4000 21 / 16, 2 x 8 heads of 128 x 50001 501 /
-  // 72. Many segments shorter than a CTA's warps are better packed (64 x 20 of 59 tokens: 17 / 12.7).
-  const long long segs = (long long)B * cache->kv_heads * passes;
+  // 256 of up to 1500 151 / 172, 16 of up to 4000 38 / 43, 4 of up to 4000 21 / 16, 2 x 8 heads of 128 x 50001 501 / 72.
+  const long long segs = (long long)B * cache->kv_heads * passes, slots = (long long)ctas * k.warps;
   const long long per_warp = (cap_tiles + k.warps - 1) / k.warps;
-  const bool seg = (per_warp <= 8 || (per_warp <= 24 && segs * 5 >= (long long)ctas * 4)) &&
-                   (segs <= ctas || cap_tiles >= k.warps) && segs <= 0x7fffffffLL;
+  const bool seg = (per_warp <= 8 || (per_warp <= 24 && segs * 5 >= (long long)ctas * 4)) && segs <= 0x7fffffffLL;
   if (seg) {
     a.B = B;
     a.table = d_page_table;
@@ -375,7 +374,14 @@ int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* 
     a.len = d_len;
     a.start = d_start;
     cudaError_t e = cudaFuncSetAttribute(k.seg, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
-    if (e == cudaSuccess) e = launch(k.seg, dim3((unsigned)segs), 32 * k.warps, k.smem, stream, a);
+    // Its warps: all of them where CTAs are few; else so many that each has about sixteen tiles, or that there are
+    // warps for the whole machine (but six tiles each): what a warp pays to begin and to end a segment is a few
+    // tiles' work (256 sequences of up to 1500 in 8-bit codes: 115 us with two, 151 with eight).
+    long long nw = k.warps;
+    if (segs > ctas)
+      nw = std::max({2LL, (cap_tiles + 15) / 16, std::min((3 * slots / 2 + segs - 1) / segs, (cap_tiles + 5) / 6)});
+    nw = std::min({nw, (long long)k.warps, cap_tiles});
+    if (e == cudaSuccess) e = launch(k.seg, dim3((unsigned)segs), (int)(32 * nw), k.smem / k.warps * nw, stream, a);
     return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "attention launch");
   }
   const int group = (int)std::min<long long>(c4s::ATT_MAXB, 0x7fffffffLL / cap_tiles);
