@@ -190,6 +190,12 @@ __device__ __forceinline__ float rows_max(float v) {
 
 // P[0..B]: exclusive prefix sums of the sequences' tiles (all threads of the
 // CTA; `red` holds one value per warp).
+// (A length past what the page table can name is cut, and reported.)
+__device__ __forceinline__ void attn_visible(const AttnArgs& a, int b, bool tell, long long& lo, long long& hi) {
+  const int len = a.len[b];
+  kv_visible(len, a.start ? a.start[b] : 0, a.max_pages, a.c.page_size, lo, hi);
+  if (tell && len > hi) atomicOr(a.errflags, C4S_DEVERR_KV_PAGE);
+}
 template <int WARPS>
 __device__ __forceinline__ void attn_prefix(const AttnArgs& a, int tok, int* P, int* red) {
   constexpr int NTH = 32 * WARPS;
@@ -200,7 +206,7 @@ __device__ __forceinline__ void attn_prefix(const AttnArgs& a, int tok, int* P, 
     int x = 0;
     if (b < a.B) {
       long long lo, hi;
-      kv_visible(a.len[b], a.start ? a.start[b] : 0, a.max_pages, a.c.page_size, lo, hi);
+      attn_visible(a, b, blockIdx.x == 0, lo, hi);
       x = (int)kv_tiles(lo, hi, tok);
     }
     int s = x;
@@ -231,7 +237,7 @@ struct AttnCursor {
   unsigned lo, hi;
   __device__ __forceinline__ void sequence(const AttnArgs& a, const int* P) {
     long long l, h;
-    kv_visible(a.len[b], a.start ? a.start[b] : 0, a.max_pages, a.c.page_size, l, h);
+    attn_visible(a, b, false, l, h);
     lo = (unsigned)l;
     hi = (unsigned)h;
     nt = P[b + 1] - P[b];
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
     look.kvh = h / QB;
     look.qb = h - look.kvh * QB;
     long long lo, hi;
-    kv_visible(a.len[look.b], a.start ? a.start[look.b] : 0, a.max_pages, a.c.page_size, lo, hi);
+    attn_visible(a, look.b, h == 0 && threadIdx.x == 0, lo, hi);
     look.lo = (unsigned)lo;
     look.hi = (unsigned)hi;
     look.nt = (int)kv_tiles(lo, hi, TOK);
@@ -340,7 +346,7 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
     if (looked++ > 0 && ++look.i == look.nt) {
       if constexpr (!SEG) look.next_segment(a, P, QB);
     }
-    const unsigned pos = look.lo + look.i * TOK + lane;
+    const unsigned pos = look.lo + (unsigned)look.i * TOK + lane;
     lk_in = lane < TOK && pos < look.hi;
     if (lk_in) {                                   // inside the table: hi is cut to its width
       const int pi = page_of(a.pdiv, (int)pos);
@@ -401,7 +407,9 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
   unsigned qf[KS][2];                              // q as the B operand: column g, k-step's four elements
   float qmul[QN], qsum[CODES ? NG : 1][QN];
   float m[QN], l[QN], o[QN][KS][4], ob[CODES ? NG : 1][QN];
-  float smax = 0.0f;                               // codes: largest value scale so far
+  // codes: largest value scale so far; not below this, whose reciprocal times 2^15 is a number
+  constexpr float SMIN = 1e-30f;
+  float smax = SMIN;
 
   auto begin_segment = [&]() {
     const int qb = cur.qb, kvh = cur.kvh;
@@ -487,7 +495,7 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
 #pragma unroll
       for (int n = 0; n < NG; ++n) ob[CODES ? n : 0][u] = 0.0f;
     }
-    smax = 0.0f;
+    smax = SMIN;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       qf[s][0] = pack2<M>(Cvt<M>::t(x[s][0]), Cvt<M>::t(x[s][1]));
@@ -610,7 +618,7 @@ __global__ void __launch_bounds__(32 * AttnCfg<D, BITS, GS, NQ>::WARPS, ATT_CTAS
         smax = ns;
         moved = true;
       }
-      sinv = smax > 0.0f || smax != smax ? PSCALE / smax : 0.0f;
+      sinv = PSCALE / smax;
     }
     if (__any_sync(FULL, moved)) {
 #pragma unroll

@@ -130,8 +130,9 @@ class GPT2Stack:
         h = h + linear(gelu(linear(LN2(h))))
 
     with the residual stream in bf16, as the head takes it. All state (lengths,
-    page table, caches, buffers) lives on the device; a call reads nothing back
-    and allocates nothing, so a step can be captured into a CUDA graph.
+    page table, caches, buffers) lives on the device and a call reads nothing
+    back, so a step can be captured into a CUDA graph. A stream that runs past
+    its `positions` is not written any further (C4S_DEVERR_KV_PAGE).
 
     layers       one dict per block of bf16 weights, out x in (a checkpoint's
                  Conv1D weights transposed), fp32 biases (or None) and norms:

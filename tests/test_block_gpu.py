@@ -398,6 +398,39 @@ def test_attention_bad_pages(ctx, c4s):
     assert (out[1, 0].double() - p @ v[1][:, 0]).abs().max() < 0.02
 
 
+@pytest.mark.parametrize("wide", [0, 4000])
+def test_attention_past_the_table(ctx, c4s, wide):
+    """A length past the page table is cut to it and reported; one that fits is not."""
+    g = gen(18)
+    cache, table = filled(c4s, [64, 40], 1, 64, 16, BF, 16, 64, g, nan=False)
+    table = torch.cat([table, table[:, :1].expand(2, wide)], 1).contiguous()
+    cap = 16 * table.shape[1]
+    q = torch.randn((2, 1, 64), generator=g, device=DEV).to(BF)
+    ctx.paged_attention(q, cache, table, i32([64, 40]))
+    assert ctx.status()[0] == 0
+    want = ctx.paged_attention(q, cache, table, i32([cap, 40]))
+    table[1] = table[0]
+    assert ctx.status()[0] == 0
+    out = ctx.paged_attention(q, cache, table, i32([cap + 1, (1 << 31) - 1]))
+    assert ctx.status(reset=True)[0] == 16
+    assert torch.equal(out[0], want[0]) and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_attention_tiny_and_huge_codes(ctx, c4s, bits):
+    """Scales near fp32's smallest numbers and near its largest, within one sequence and all along it."""
+    g = gen(19)
+    lens = [100, 100, 100]
+    cache, table = filled(c4s, lens, 2, 64, 16, BF, bits, 64, g)
+    q = torch.randn((3, 2, 64), generator=g, device=DEV).to(BF)
+    cache.v_sb[table[0, :7].long()] *= 2.0 ** -112
+    cache.v_sb[table[1, :7].long()] *= 2.0 ** 100
+    cache.v_sb[table[2, 2].long()] *= 2.0 ** 60
+    cache.v_sb[table[2, 4].long()] *= 2.0 ** -100
+    out = ctx.paged_attention(q, cache, table, i32(lens))
+    check_attention(ctx, c4s, q, cache, table, lens, None, 0.125, out)
+
+
 @pytest.mark.parametrize("wide", [0, 5000])
 def test_attention_repeats_and_graphs(ctx, c4s, wide):
     """The same call gives the same bits; two graphs with workspaces of their own, replayed on two streams while
