@@ -163,6 +163,9 @@ __device__ __forceinline__ float4 ld_cluster(unsigned addr, unsigned rank) {
   return v;
 }
 
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(map)) : "memory");
+}
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
                    reinterpret_cast<unsigned long long>(map)),
@@ -210,6 +213,8 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
   const int KB = (a.K + LN_BK - 1) / LN_BK;
   const int k0 = (int)((long long)KB * s / S), k1 = (int)((long long)KB * (s + 1) / S);
   if (threadIdx.x == 0) {
+    tma_prefetch_map(&tmX);
+    tma_prefetch_map(&tmW);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -360,6 +365,7 @@ constexpr unsigned LP_HALF = 128 * LN_BK * 2;      // 16 KB: a CTA's rows of x o
 // by TMA, whole lines at once: 16-byte stores of one row a lane took 41 us of a
 // 49 us product (4099 x 1280 -> 5120).
 constexpr unsigned LP_OUT = 32 * 128;
+constexpr long long LP_AHEAD = 48 << 20;           // bytes of a weight that is read ahead into L2 (126 MB)
 // Sixteen epilogue warps hide the activation's latency best (GELU: 42.5 us
 // there, 45.2 with eight); fp32 outputs take more registers than those leave.
 // BN 128: half the columns, for batches whose 256-wide tiles would leave SMs
@@ -425,6 +431,9 @@ __global__ void __launch_bounds__(LpCfg<TO, BN>::THREADS, 1) lin_pair_kernel(con
   const int mt = (a.M + 255) / 256, nt = (a.N + BN - 1) / BN;
   const long long tiles = (long long)mt * nt;
   if (threadIdx.x == 0) {
+    tma_prefetch_map(&tmX);
+    tma_prefetch_map(&tmW);
+    if (a.vec_out) tma_prefetch_map(&tmO);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -447,6 +456,12 @@ __global__ void __launch_bounds__(LpCfg<TO, BN>::THREADS, 1) lin_pair_kernel(con
   cluster_wait();
   tc_fence_after();
   const unsigned tmem = tmem_base;
+  // the weight on its way to L2 (a share of its tiles from every CTA) while the norm before this kernel still runs
+  if (warp == 0 && (long long)a.N * a.K * 2 <= LP_AHEAD) {
+    const int boxes = (a.N + BN / 2 - 1) / (BN / 2) * KB;
+    for (int i = blockIdx.x + gridDim.x * lane; i < boxes; i += gridDim.x * 32)
+      tma_prefetch_2d(&tmW, i % KB * LN_BK, i / KB * (BN / 2));
+  }
   grid_dep_wait();
   grid_dep_launch();
   auto give_up = [&]() {
