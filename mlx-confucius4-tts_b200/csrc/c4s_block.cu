@@ -179,14 +179,14 @@ struct TilePick {
   int stages;
 };
 // one CTA a tile, a ring of up to `room` bytes for x boxes of xbytes
-template <typename TI, typename TO> TilePick tile_pick(int bn, unsigned xbytes, size_t room) {
+template <typename TI, typename TO> TilePick tile_pick(int bn, unsigned xbytes, size_t room, int rows) {
   TilePick p;
   if (bn == 64) {
     p.kern = c4s::lin_tile_kernel<TI, TO, 64>;
-    c4s::LinCfg<64>::ring(xbytes, room, p.stages, p.smem);
+    c4s::LinCfg<64>::plan(xbytes, room, rows, p.stages, p.smem);
   } else {
     p.kern = c4s::lin_tile_kernel<TI, TO, 128>;
-    c4s::LinCfg<128>::ring(xbytes, room, p.stages, p.smem);
+    c4s::LinCfg<128>::plan(xbytes, room, rows, p.stages, p.smem);
   }
   return p;
 }
@@ -450,7 +450,9 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
   a.errflags = ctx->d_err;
   a.vec_bias = ((uintptr_t)d_bias & 15) == 0;
   a.xbytes = 0;
-  if (M <= c4s::LF_ROWS) {
+  // few rows: the weight through the warps; long K better by tiles and clusters (us, warps / tiles: 1 x 1280 -> 1280
+  // 3.3 / 4.4, 8 x 2560 -> 1280 5.0 / 5.2, 1 x 5120 -> 1280 7.5 / 6.1, 8 x 8192 -> 4096 16.2 / 12.7)
+  if (M <= c4s::LF_ROWS && K < 4096) {
     const bool f32 = out_dtype == C4S_FP32, norm = d_norm != nullptr;
     e = dtype == C4S_BF16
             ? (f32 ? launch_few<__nv_bfloat16, float>(ctx, d_x, ld_x, d_gamma, d_beta, eps, norm, d_weight, ld_weight, a, stream)
@@ -499,10 +501,12 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
   const size_t room = bn == 128 || nt * mt * S <= ctx->num_sms ? 225 * 1024 : 112 * 1024;
   if (!encode_rows(&tx, dtype, d_x, K, M, ld_x * 2, box) || !encode_rows(&tw, dtype, d_weight, K, N, ld_weight * 2, bn))
     return fail(ctx, C4S_ERR_CUDA, "tensor map encoding failed");
-  const TilePick k = dtype == C4S_BF16 ? (f32 ? tile_pick<__nv_bfloat16, float>(bn, a.xbytes, room)
-                                              : tile_pick<__nv_bfloat16, __nv_bfloat16>(bn, a.xbytes, room))
-                                       : (f32 ? tile_pick<__half, float>(bn, a.xbytes, room)
-                                              : tile_pick<__half, __half>(bn, a.xbytes, room));
+  // rows of partials that a CTA of a cluster gathers: its share of the tile's rows from every CTA
+  const int parts = S > 1 ? S * ((std::min(c4s::LN_BM, M) + S - 1) / S) : 0;
+  const TilePick k = dtype == C4S_BF16 ? (f32 ? tile_pick<__nv_bfloat16, float>(bn, a.xbytes, room, parts)
+                                              : tile_pick<__nv_bfloat16, __nv_bfloat16>(bn, a.xbytes, room, parts))
+                                       : (f32 ? tile_pick<__half, float>(bn, a.xbytes, room, parts)
+                                              : tile_pick<__half, __half>(bn, a.xbytes, room, parts));
   e = launch_cluster(k.kern, dim3((unsigned)(nt * S), (unsigned)mt), S, c4s::LN_THREADS, k.smem, stream, tx, tw, a, S,
                      k.stages);
   return e == cudaSuccess ? C4S_OK : cuda_fail(ctx, e, "linear launch");

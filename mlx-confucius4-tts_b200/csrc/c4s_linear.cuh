@@ -11,8 +11,10 @@
 // warp, one MMA-issuing lane, eight epilogue warps; a ring of 64-wide k-blocks
 // in 128-byte-swizzled shared memory, the accumulator in TMEM). Where the
 // tiles are fewer than the SMs, a cluster of S CTAs shares a tile: each takes
-// a part of K, leaves its fp32 partial in its own shared memory, and sums a
-// share of the rows over the cluster in a fixed order.
+// a part of K, and a share of the rows, whose fp32 partials the others put into
+// its shared memory; it sums them in a fixed order. (Reading the others'
+// partials instead takes a second barrier, so that none leaves early, and the
+// loads' latency: 9.1 us against 8.1 at 64 x 5120 -> 1280.)
 // lin_pair_kernel: 256 x 256 tiles by pairs of CTAs, for large products.
 // lin_few_kernel: few rows of x, the weight streamed once, no TMEM.
 #pragma once
@@ -149,18 +151,54 @@ __device__ __forceinline__ void lin_store(const LinArgs& a, long long row, int n
   }
 }
 
+// Four outputs of a row: 8- or 16-byte stores where the row allows them.
+template <typename TO>
+__device__ __forceinline__ void lin_store4(const LinArgs& a, long long row, int n, float (&v)[4]) {
+  TO* o = static_cast<TO*>(a.out) + row * a.ldo + n;
+  const bool full = n + 4 <= a.N;
+  __align__(16) TO x[4];
+  using Vec = typename std::conditional<sizeof(TO) == 2, uint2, uint4>::type;
+  if (a.residual) {
+    const TO* r = static_cast<const TO*>(a.residual) + row * a.ldr + n;
+    if (full && a.vec_res) {
+      *reinterpret_cast<Vec*>(x) = *reinterpret_cast<const Vec*>(r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = n + i < a.N ? r[i] : Cvt<TO>::t(0.0f);
+    }
+  }
+  if (a.bias) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.N) v[i] += __ldg(a.bias + n + i);
+  }
+  activate(v, a.act);
+  if (a.residual)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += Cvt<TO>::f(x[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = Cvt<TO>::t(v[i]);
+  if (full && a.vec_out) {
+    *reinterpret_cast<Vec*>(o) = *reinterpret_cast<const Vec*>(x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.N) o[i] = x[i];
+  }
+}
+
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void umma_commit_at(unsigned bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ float4 ld_cluster(unsigned addr, unsigned rank) {
+__device__ __forceinline__ unsigned map_rank(unsigned addr, unsigned rank) {
   unsigned p;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(p) : "memory");
-  return v;
+  return p;
+}
+__device__ __forceinline__ void st_cluster(unsigned addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
@@ -183,14 +221,16 @@ template <int BN>
 struct LinCfg {
   static constexpr unsigned WB = BN * LN_BK * 2;                           // bytes of a W tile
   static constexpr int PPITCH = BN + 4;                                    // floats per row of a split tile's partial
-  static constexpr size_t SLACK = LN_BM * LN_BK * 2;
-  static constexpr size_t FLOOR = (size_t)LN_BM * PPITCH * 4;              // a split tile's partial
-  // stages and bytes of shared memory for boxes of xbytes, `room` bytes at most
-  static void ring(unsigned xbytes, size_t room, int& st, size_t& smem) {
-    st = (int)((room - SLACK - 1024) / (WB + xbytes));
+  static constexpr unsigned FULL_BOX = LN_BM * LN_BK * 2;
+  // bytes of a ring of st stages with the slack behind it
+  static __host__ __device__ unsigned ring_bytes(int st, unsigned xbytes) { return (unsigned)st * (WB + xbytes) + FULL_BOX - xbytes; }
+  // stages and bytes of shared memory for boxes of xbytes, `room` bytes at most; behind the ring the partials of
+  // `rows` rows (0: not split), which arrive while this CTA's ring may still be in use
+  static void plan(unsigned xbytes, size_t room, int rows, int& st, size_t& smem) {
+    const size_t parts = (size_t)rows * PPITCH * 4;
+    st = (int)((room - 1024 - parts - (FULL_BOX - xbytes)) / (WB + xbytes));
     st = st < 2 ? 2 : st > LT_MAX_ST ? LT_MAX_ST : st;
-    smem = (size_t)st * (WB + xbytes) + SLACK;
-    smem = (smem > FLOOR ? smem : FLOOR) + 1024;
+    smem = ring_bytes(st, xbytes) + parts + 1024;
   }
 };
 
@@ -210,6 +250,9 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
   const int warp = __shfl_sync(FULL, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // known to be uniform
   const int s = (int)(blockIdx.x % (unsigned)S);
   const int n0 = (int)(blockIdx.x / (unsigned)S) * BN, m0 = blockIdx.y * LN_BM;
+  const int rows = min(LN_BM, a.M - m0);           // of the tile
+  const unsigned ring_bytes = Cfg::ring_bytes(ST, a.xbytes);
+  const unsigned parts = smem_u32(ring) + ring_bytes;          // the others' partials of this CTA's rows
   const int KB = (a.K + LN_BK - 1) / LN_BK;
   const int k0 = (int)((long long)KB * s / S), k1 = (int)((long long)KB * (s + 1) / S);
   if (threadIdx.x == 0) {
@@ -230,6 +273,7 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = tmem_base;
+  if (S > 1) cluster_arrive();                     // waited for before the first store into another CTA
   // the weight's tiles on their way to L2 while the kernel before this one still runs
   if (warp == 0 && lane < k1 - k0) tma_prefetch_2d(&tmW, (k0 + lane) * LN_BK, n0);
   grid_dep_wait();                                 // x (the norm's output among it) and the residual
@@ -288,26 +332,28 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
     if (!ok) give_up();
     tc_fence_after();
     __syncwarp();
+    if (S > 1) cluster_wait();
     const int q = warp & 3, half = (warp - 2) >> 2;           // TMEM lane quarter; which column chunks
-    const int rows = min(LN_BM, a.M - m0);
     if (ok && !abort_flag && k1 > k0 && 32 * q < rows) {
+      const int r = 32 * q + lane;
+      // the CTA that sums row r, and where this CTA's part of the row goes there: [rank][its rows][PPITCH]
+      const int o = r < rows ? ((r + 1) * S - 1) / rows : 0, o0 = rows * o / S, on = rows * (o + 1) / S - o0;
+      const unsigned dst = S > 1 ? map_rank(parts, (unsigned)o) + (unsigned)((s * on + r - o0) * Cfg::PPITCH) * 4u : 0u;
       for (int c = half; c < BN / 32; c += 2) {
-        const unsigned taddr = tmem + ((unsigned)(32 * q) << 16) + (unsigned)(32 * c);
         float v[32];
-        tmem_ld32(taddr, reinterpret_cast<unsigned(&)[32]>(v));
+        tmem_ld32(tmem + ((unsigned)(32 * q) << 16) + (unsigned)(32 * c), reinterpret_cast<unsigned(&)[32]>(v));
         tmem_ld_wait();
+        if (r >= rows) continue;
         if (S == 1) {
-          if (m0 + 32 * q + lane < a.M && n0 + 32 * c < a.N)
-            lin_store<TO, 32>(a, (long long)m0 + 32 * q + lane, n0 + 32 * c, v);
+          if (n0 + 32 * c < a.N) lin_store<TO, 32>(a, (long long)m0 + r, n0 + 32 * c, v);
         } else {
-          float* p = reinterpret_cast<float*>(ring) + (32 * q + lane) * Cfg::PPITCH + 32 * c;
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          for (int j = 0; j < 32; j += 4) st_cluster(dst + (unsigned)(32 * c + j) * 4u, v[j], v[j + 1], v[j + 2], v[j + 3]);
         }
       }
     }
   }
+  if (S > 1 && warp < 2) cluster_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -315,39 +361,24 @@ __global__ void __launch_bounds__(LN_THREADS, BN <= 64 ? 2 : 1) lin_tile_kernel(
     tmem_dealloc(tmem, BN);
   }
   if (S > 1) {
-    // every CTA of the cluster passes both barriers, also after a wait that gave up
+    // (a CTA whose wait gave up passes here too, and its rows are reported as not to be trusted)
     cluster_arrive();
+    constexpr int CG = BN / 4;                     // four columns a thread
+    const int r0 = rows * s / S, rn = rows * (s + 1) / S - r0;
+    const float* part = reinterpret_cast<const float*>(ring + ring_bytes);
     cluster_wait();
-    const int rows = min(LN_BM, a.M - m0);
-    const int r0 = rows * s / S, r1 = rows * (s + 1) / S;     // this CTA's share of the rows
-    constexpr int NV = 16 / sizeof(TO), CG = BN / NV;         // NV columns a thread
-    if (!abort_flag) {
-      for (int i = threadIdx.x; i < (r1 - r0) * CG; i += LN_THREADS) {
-        const int r = r0 + i / CG, c = (i % CG) * NV;
-        if (n0 + c >= a.N) continue;
-        float v[NV];
+    for (int i = threadIdx.x; i < rn * CG; i += LN_THREADS) {
+      const int r = i / CG, c = (i % CG) * 4, n = n0 + c;
+      if (n >= a.N) continue;
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int j = 0; j < NV; ++j) v[j] = 0.0f;
-        const unsigned addr = smem_u32(ring) + (unsigned)(r * Cfg::PPITCH + c) * 4u;
-#pragma unroll
-        for (int j = 0; j < NV; j += 4) {
-          float4 x[LN_MAX_SPLIT];                  // all on their way before any is added
-#pragma unroll
-          for (int p = 0; p < LN_MAX_SPLIT; ++p)
-            x[p] = p < S ? ld_cluster(addr + 4u * j, (unsigned)p) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-          for (int p = 0; p < LN_MAX_SPLIT; ++p) {
-            v[j] += x[p].x;
-            v[j + 1] += x[p].y;
-            v[j + 2] += x[p].z;
-            v[j + 3] += x[p].w;
-          }
+      for (int p = 0; p < LN_MAX_SPLIT; ++p)
+        if (p < S) {
+          const float4 x = *reinterpret_cast<const float4*>(part + (p * rn + r) * Cfg::PPITCH + c);
+          v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
         }
-        lin_store<TO, NV>(a, (long long)m0 + r, n0 + c, v);
-      }
+      lin_store4<TO>(a, (long long)m0 + r0 + r, n, v);
     }
-    cluster_arrive();
-    cluster_wait();                                // no CTA leaves while another reads its partial
   }
 }
 
@@ -380,11 +411,6 @@ struct LpCfg {
   static constexpr size_t SMEM = ST * (size_t)STAGE + EPI * (size_t)LP_OUT + 1024;
 };
 
-__device__ __forceinline__ unsigned map_rank(unsigned addr, unsigned rank) {
-  unsigned p;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
-  return p;
-}
 // A tile into this CTA's memory, counted on a barrier of the pair's first CTA.
 __device__ __forceinline__ void tma_load_pair(unsigned dst, const CUtensorMap* map, int x, int y, unsigned bar) {
   asm volatile(
@@ -668,7 +694,8 @@ __global__ void __launch_bounds__(LNORM_NT) lin_norm_kernel(const T* __restrict_
 
 // ---- few rows: the weight streamed once through the warps --------------------
 // Decode steps of up to 8 streams read the whole weight for a few rows of x:
-// bound by HBM, and by latency at these sizes (13 MB take 2 us). One CTA takes
+// bound by HBM, and by latency at these sizes (10 MB take 1.5 us; 1 x 1280 ->
+// 3840 takes 4.9 us, 6.9 with the LayerNorm). One CTA takes
 // R rows of W, its WARPS warps interleaved 64-wide pieces of K: every 16-byte
 // load of W goes straight into the A fragments of mma.m16n8k16 (the order of K
 // inside a piece is the same for W and x, so no shuffle is needed), x's rows

@@ -89,8 +89,9 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// The same for a warp that feeds a pipeline, on a shared-memory address: a
-// tight loop first, the timer only after many tries.
+// The same for a whole converged warp that feeds a pipeline, on a
+// shared-memory address: a tight loop first, the timer only after many tries.
+// Every lane gets the same answer.
 __device__ __forceinline__ bool mbar_wait_hot(unsigned bar, unsigned parity) {
   unsigned ok;
   asm volatile(
@@ -107,7 +108,7 @@ __device__ __forceinline__ bool mbar_wait_hot(unsigned bar, unsigned parity) {
       : "=r"(ok)
       : "r"(bar), "r"(parity)
       : "memory");
-  if (ok) return true;
+  if (__all_sync(FULL, ok)) return true;
   const unsigned long long t0 = globaltimer_ns();
   for (unsigned it = 0; it < (1u << 30); ++it) {
     asm volatile(
@@ -117,8 +118,8 @@ __device__ __forceinline__ bool mbar_wait_hot(unsigned bar, unsigned parity) {
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
-    if (ok) return true;
-    if ((it & 63u) == 63u && globaltimer_ns() - t0 > 1000000000ull) return false;
+    if (__all_sync(FULL, ok)) return true;
+    if (__any_sync(FULL, (it & 63u) == 63u && globaltimer_ns() - t0 > 1000000000ull)) return false;
   }
   return false;
 }
