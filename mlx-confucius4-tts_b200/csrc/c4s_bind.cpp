@@ -398,6 +398,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor* norm_out = a.maybe("norm_out");
     const Tensor* out = a.maybe("out");
     const LinCall r = linear_ok(x, w, bias, residual, gamma, beta, out, dtype_arg(a, x));
+    if (!norm && (gamma || beta)) value_error("gamma and beta are the LayerNorm's: layer_norm=True");
     if (norm_out) {
       matrix_ok(*norm_out, "norm_out", r.M, r.K);
       if (norm_out->scalar_type() != x.scalar_type() || !norm_out->is_contiguous())

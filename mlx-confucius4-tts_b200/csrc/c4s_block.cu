@@ -417,6 +417,7 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
   if (act < C4S_ACT_NONE || act > C4S_ACT_RELU) return fail(ctx, C4S_ERR_INVALID, "unknown activation");
   if (M == 0) return C4S_OK;
   if (!d_x || !d_weight || !d_out) return fail(ctx, C4S_ERR_INVALID, "null pointer");
+  if (d_out == d_x || d_out == d_weight) return fail(ctx, C4S_ERR_INVALID, "out must not be x or the weight");
   if (M == 1) {                                    // one row: its stride says nothing
     ld_x = K;
     ld_out = ld_residual = 0;

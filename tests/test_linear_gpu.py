@@ -187,4 +187,9 @@ def test_c_refusals(ctx, c4s):
         ctx.linear(big, big, layer_norm=True)
     with pytest.raises(ValueError):
         ctx.linear(x.cpu(), x)
+    with pytest.raises(ValueError):
+        ctx.linear(x, x, gamma=torch.ones(64, device=DEV))           # a norm's scale without the norm
+    sq = torch.zeros((64, 64), dtype=BF, device=DEV)
+    with pytest.raises(c4s.C4SError):
+        ctx.linear(sq, sq.clone(), out=sq)                           # its own input
     assert ctx.status()[0] == 0
