@@ -238,7 +238,8 @@ int c4s_qgemv(c4s_ctx* ctx, const float* d_x, int32_t B, int32_t K, const uint32
  *             k_sb / v_sb (same addressing, strides of its own): value =
  *             scale code + bias. The code is the integer nearest to
  *             (x - min) (2^bits - 1) / (max - min), ties to even, decided
- *             exactly; a group with a NaN or infinity reads back as NaN.
+ *             exactly (an element 2^40 below the group's largest counts as
+ *             zero there); a group with a NaN or infinity reads back as NaN.
  * k and v share the strides. head_dim 64, 96 or 128, divided by the group;
  * row addresses and strides multiples of 16 bytes, of pairs 8 bytes.
  *

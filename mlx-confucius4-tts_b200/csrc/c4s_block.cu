@@ -94,7 +94,7 @@ int kv_args(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* table, int64
   const uintptr_t es = dtype == C4S_FP32 ? 4 : 2;
   if (((uintptr_t)k | (uintptr_t)v) & (es - 1)) return fail(ctx, C4S_ERR_INVALID, "misaligned rows");
   a.units = cache->kv_heads * (cache->head_dim / 8);
-  a.per_cta = std::max(1, std::min(c4s::KV_TOKS, c4s::KV_UNITS / a.units));
+  a.per_cta = std::max(1, std::min(c4s::KV_TOKS, (cache->bits == 16 ? c4s::KV_UNITS16 : c4s::KV_UNITS) / a.units));
   // few tokens: spread over the SMs
   while (a.per_cta > 1 && (T + a.per_cta - 1) / a.per_cta < 4LL * ctx->num_sms) a.per_cta = (a.per_cta + 1) / 2;
   const long long ctas = (T + a.per_cta - 1) / a.per_cta;
