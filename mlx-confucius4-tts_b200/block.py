@@ -7,7 +7,8 @@ defines each operator.
 Arguments are checked by the compiled binding (ValueError, TypeError) before
 the C call, whose own refusals raise C4SError. Calls are ordered on the current
 torch stream of the context's device, or on `stream`; with `stream` the outputs
-that a call allocates belong to that stream.
+that a call allocates belong to that stream. The operators are for inference:
+what they write has no gradient.
 """
 from __future__ import annotations
 
@@ -88,6 +89,8 @@ class KVCache:
             raise ValueError("bits must be 16, 8 or 4")
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
             raise ValueError("k and v must be alike, [pages, kv_heads, page_size, row]")
+        if min(k.shape) < 1:
+            raise ValueError("a cache has at least one page, slot and head")
         if k.stride(3) != 1:
             raise ValueError("cache rows must be contiguous")
         self.k, self.v, self.k_sb, self.v_sb, self.bits = k, v, k_sb, v_sb, bits

@@ -69,6 +69,13 @@ def test_cache_refusals():
         K.empty(4, 16, 2, 96, bits=8, group=64, device="cpu")
 
 
+def test_cache_without_heads_or_pages():
+    K = load_c4s().KVCache
+    for shape in ((4, 0, 16, 64), (0, 2, 16, 64), (4, 2, 0, 64)):
+        with pytest.raises(ValueError):
+            K(torch.zeros(shape, dtype=torch.bfloat16), torch.zeros(shape, dtype=torch.bfloat16))
+
+
 def test_call_refusals():
     c4s = load_c4s()
     b = c4s.block

@@ -343,6 +343,18 @@ def test_attention_many_sequences(ctx, c4s, wide):
     check_attention(ctx, c4s, q, cache, table, lens, None, 0.125, out)
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-6])
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_attention_scales(ctx, c4s, scale, bits):
+    """Scales below zero, zero (the mean of the values) and near it."""
+    g = gen(23)
+    lens = [70, 1, 33]
+    cache, table = filled(c4s, lens, 2, 64, 16, BF, bits, 64, g)
+    q = torch.randn((3, 4, 64), generator=g, device=DEV).to(BF)
+    out = ctx.paged_attention(q, cache, table, i32(lens), scale=scale)
+    check_attention(ctx, c4s, q, cache, table, lens, None, scale, out)
+
+
 def test_attention_strides_scale_and_out(ctx, c4s):
     """Queries as a slice of a fused projection, at odd offsets; outputs into a slice, the rest left as it was."""
     g = gen(11)
