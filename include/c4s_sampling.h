@@ -310,7 +310,7 @@ int c4s_paged_attention(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* 
  *   d_x       [M, ld_x] bf16 or fp16 (dtype), K elements a row
  *   d_norm    [M, K] of dtype, 16-byte aligned: caller-owned workspace of the
  *             normalised rows (rounded to dtype, the product's operand;
- *             contents undefined afterwards), with d_gamma, d_beta fp32 [K] or
+ *             contents undefined afterwards; no other argument), with d_gamma, d_beta fp32 [K] or
  *             NULL (1, 0) and eps; NULL skips the LayerNorm
  *   d_weight  [N, ld_weight] of dtype (out x in)
  *   d_bias    fp32 [N] or NULL;  act: C4S_ACT_*

@@ -418,9 +418,11 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
   if (M == 0) return C4S_OK;
   if (!d_x || !d_weight || !d_out) return fail(ctx, C4S_ERR_INVALID, "null pointer");
   if (d_out == d_x || d_out == d_weight) return fail(ctx, C4S_ERR_INVALID, "out must not be x or the weight");
+  if (d_norm && (d_norm == d_x || d_norm == d_weight || d_norm == d_residual || d_norm == d_out))
+    return fail(ctx, C4S_ERR_INVALID, "the LayerNorm's workspace must be its own");
   if (M == 1) {                                    // one row: its stride says nothing
     ld_x = K;
-    ld_out = ld_residual = 0;
+    ld_out = ld_residual = ((int64_t)N + 7) / 8 * 8;
   }
   if (N == 1) ld_weight = K;
   if ((M > 1 && (ld_x < K || ld_out < N || (d_residual && ld_residual < N))) || ld_weight < K)
@@ -451,6 +453,7 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
   a.errflags = ctx->d_err;
   a.vec_bias = ((uintptr_t)d_bias & 15) == 0;
   a.xbytes = 0;
+  a.whole = 0;
   // few rows: the weight through the warps; long K better by tiles and clusters (us, warps / tiles: 1 x 1280 -> 1280
   // 3.3 / 4.4, 8 x 2560 -> 1280 5.0 / 5.2, 1 x 5120 -> 1280 7.5 / 6.1, 8 x 8192 -> 4096 16.2 / 12.7)
   if (M <= c4s::LF_ROWS && K < 4096) {
@@ -477,11 +480,14 @@ int c4s_linear(c4s_ctx* ctx, const void* d_x, int32_t dtype, int32_t M, int32_t 
     // pairs of CTAs on 256 x 256 tiles where those fill the machine, on 256 x 128 where those fill half of it
     // (256 x 1280 -> 5120: 10.3 us by single CTAs on 160 tiles)
     const bool wide = big * 2 >= ctx->num_sms;
+    // the output's tensor map: TMA writes the last 16 bytes of a row whole, so that a row that ends inside them has
+    // its last block of 32 columns written by plain stores
+    a.whole = !a.vec_out ? 0 : N * (long long)os % 16 ? N / 32 * 32 : N;
     CUtensorMap to;
     memset(&to, 0, sizeof(to));
     if (!encode_rows(&tx, dtype, d_x, K, M, ld_x * 2, 128) ||
         !encode_rows(&tw, dtype, d_weight, K, N, ld_weight * 2, wide ? 128 : 64) ||
-        (a.vec_out && !encode_rows(&to, out_dtype, d_out, N, M, ld_out * (long long)os, 32)))
+        (a.whole > 0 && !encode_rows(&to, out_dtype, d_out, a.whole, M, ld_out * (long long)os, 32)))
       return fail(ctx, C4S_ERR_CUDA, "tensor map encoding failed");
     const PairPick k = dtype == C4S_BF16 ? (f32 ? pair_pick<__nv_bfloat16, float>(wide) : pair_pick<__nv_bfloat16, __nv_bfloat16>(wide))
                                          : (f32 ? pair_pick<__half, float>(wide) : pair_pick<__half, __half>(wide));

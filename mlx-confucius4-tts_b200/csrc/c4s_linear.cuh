@@ -68,6 +68,7 @@ struct LinArgs {
   long long ldo;
   int M, N, K;
   int act;                                         // C4S_ACT_*
+  int whole;                                       // columns that the output's tensor map has
   bool vec_out, vec_res, vec_bias;                 // 16-byte aligned rows (from columns that are multiples of 32)
   unsigned xbytes;                                 // bytes of one TMA box of x
   unsigned* errflags;
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(LpCfg<TO, BN>::THREADS, 1) lin_pair_kernel(con
   if (threadIdx.x == 0) {
     tma_prefetch_map(&tmX);
     tma_prefetch_map(&tmW);
-    if (a.vec_out) tma_prefetch_map(&tmO);
+    if (a.whole > 0) tma_prefetch_map(&tmO);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -565,7 +566,6 @@ __global__ void __launch_bounds__(LpCfg<TO, BN>::THREADS, 1) lin_pair_kernel(con
       tc_fence_after();
       if (!__all_sync(FULL, ok) || abort_flag) break;
       const unsigned taddr = tmem + ((unsigned)(32 * q) << 16) + (unsigned)(buf * BN + CW * cg);
-      const bool tma = a.vec_out;                  // rows that a tensor map can name
       constexpr int PER = 16 / sizeof(TO), PIECES = 32 / PER;  // 16-byte pieces of a row's 32 columns
       constexpr bool ONE = PIECES == 4;            // both halves of the 64 columns make one block
 #pragma unroll 1
@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(LpCfg<TO, BN>::THREADS, 1) lin_pair_kernel(con
           }
         }
         if (n0 + 32 * c >= a.N || m0 >= a.M) continue;         // uniform
-        if (!tma) {
+        if (n0 + 32 * c >= a.whole) {              // not in the tensor map
           if (m0 + lane < a.M) lin_store<TO, 32>(a, m0 + lane, n0 + 32 * c, v);
           continue;
         }
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(LpCfg<TO, BN>::THREADS, 1) lin_pair_kernel(con
           const unsigned at = row + ((((ONE ? 4 * (c & 1) : 0) + i) ^ (lane & 7)) << 4);
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
         }
-        if (!ONE || c % 2 == 1 || n0 + 32 * c + 32 >= a.N) {
+        if (!ONE || c % 2 == 1 || n0 + 32 * c + 32 >= a.whole) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {

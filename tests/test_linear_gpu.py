@@ -174,6 +174,36 @@ def test_repeats_streams_and_graphs(ctx):
     assert ctx.linear(x[:0], w).shape == (0, 1280)
 
 
+@pytest.mark.parametrize("N", [19200, 20001])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_one_row_of_a_long_product(ctx, N, dtype):
+    """One row with K and N so long that the tiles of SM pairs take it: its strides say nothing."""
+    g = torch.Generator(device=DEV).manual_seed(N)
+    x = torch.randn((1, 4096), generator=g, device=DEV).to(BF)
+    w = (torch.randn((N, 4096), generator=g, device=DEV) / 64).to(BF)
+    bias = torch.randn(N, generator=g, device=DEV)
+    res = torch.randn((1, N), generator=g, device=DEV).to(dtype)
+    room = torch.full((2, N + 8), 3.0, device=DEV).to(dtype)
+    out = ctx.linear(x, w, bias, residual=res, out=room[:1, :N], out_dtype=dtype)
+    check(ctx, x, w, out, bias, residual=res)
+    assert torch.all(room[0, N:] == 3) and torch.all(room[1] == 3)
+
+
+@pytest.mark.parametrize("M,N", [(700, 2531), (513, 4097), (300, 1284), (19000, 5), (19000, 11)])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_padded_rows_of_large_products(ctx, M, N, dtype):
+    """Rows of a 16-byte pitch whose last columns end inside 16 bytes: what lies behind them is left as it was."""
+    g = torch.Generator(device=DEV).manual_seed(N)
+    x = torch.randn((M, 128), generator=g, device=DEV).to(BF)
+    w = (torch.randn((N, 128), generator=g, device=DEV) / 11).to(BF)
+    room = torch.full((M + 1, (N + 23) // 8 * 8), 3.0, device=DEV).to(dtype)
+    res = torch.randn((M, N), generator=g, device=DEV).to(dtype)
+    room[:M, :N] = res
+    out = ctx.linear(x, w, act="silu", residual=room[:M, :N], out=room[:M, :N], out_dtype=dtype)
+    check(ctx, x, w, out, None, "silu", residual=res)
+    assert torch.all(room[:, N:] == 3) and torch.all(room[M] == 3)
+
+
 def test_c_refusals(ctx, c4s):
     x = torch.zeros((4, 64), dtype=BF, device=DEV)
     with pytest.raises(c4s.C4SError):
@@ -192,4 +222,8 @@ def test_c_refusals(ctx, c4s):
     sq = torch.zeros((64, 64), dtype=BF, device=DEV)
     with pytest.raises(c4s.C4SError):
         ctx.linear(sq, sq.clone(), out=sq)                           # its own input
+    for shared in ("out", "residual", "x"):
+        t = {n: torch.zeros((64, 64), dtype=BF, device=DEV) for n in ("x", "out", "residual")}
+        with pytest.raises(c4s.C4SError):
+            ctx.linear(weight=sq, layer_norm=True, norm_out=t[shared], **t)
     assert ctx.status()[0] == 0
